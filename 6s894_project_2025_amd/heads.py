@@ -1,0 +1,204 @@
+"""Query and key heads between a projection and attention: per-head RMS norm, position rotation and
+the Hadamard rotation of the head in one pass (``include/mi_hadamard.h``: ``mi_qk_norm_rope``).
+
+Like the other ops of the package these record no autograd graph: the gradients are a function of
+their own, and a differentiable input under an active grad mode is an error rather than a silent
+detach (call them under ``torch.no_grad()`` or inside a ``torch.autograd.Function``).
+"""
+from __future__ import annotations
+
+import struct
+
+import torch
+
+from . import _lib
+from .ops import _DTYPE_CODE, _dense16, _is_pow2, _on_device_of, _require_cuda, _stream
+
+_NEIGHBOURS, _HADAMARD = 1, 2
+_HEADS = struct.Struct("<Q6Q6Q4I" "I4I" "iiIII" "f4x")  # mi_heads
+_MAX_D = 512
+
+
+def _no_graph(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} records no autograd graph: call it under torch.no_grad() or inside a "
+                           f"torch.autograd.Function, and {name}_backward for the gradients")
+
+
+def _head_strides(t: torch.Tensor) -> tuple[int, int]:
+    """Token and head stride in elements; 0 along an axis of one entry, whose stride means nothing."""
+    return (t.stride(0) if t.size(0) > 1 else 0, t.stride(1) if t.size(1) > 1 else 0)
+
+
+def _laid_out(t: torch.Tensor) -> bool:
+    """Heads contiguous, 16-byte aligned base and strides: what the kernels address directly."""
+    e = t.element_size()
+    return (t.numel() == 0 or
+            (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in _head_strides(t))))
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    return t if _laid_out(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _describe(name, q, k, q_weight, k_weight, positions, inv_freq, eps, sections, interleaved, hadamard):
+    """Checks the operands that both directions share; returns (D, R, flags, axes, section ends)."""
+    for t, n in ((q, "q"), (k, "k")):
+        if t.dim() != 3:
+            raise RuntimeError(f"{n} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
+    if q.dtype not in _DTYPE_CODE or k.dtype != q.dtype:
+        raise RuntimeError(f"q and k must share a dtype in fp32/bf16/fp16 (got {q.dtype}, {k.dtype})")
+    T, _, D = q.shape
+    if k.size(0) != T or k.size(2) != D:
+        raise RuntimeError(f"shape mismatch: q {tuple(q.shape)} k {tuple(k.shape)}")
+    if D % 16 or not 16 <= D <= _MAX_D:
+        raise RuntimeError(f"head_dim must be a multiple of 16 in [16, {_MAX_D}], got {D}")
+    if hadamard and not _is_pow2(D):
+        raise RuntimeError(f"hadamard needs a power-of-two head_dim, got {D}")
+    if not eps >= 0.0:
+        raise RuntimeError(f"eps must not be negative, got {eps}")
+    if inv_freq.dim() != 1 or inv_freq.dtype not in (torch.float32, torch.float64):
+        raise RuntimeError("inv_freq must be a vector in fp32 or fp64")
+    half = inv_freq.numel()
+    if half % 8 or 2 * half > D:
+        raise RuntimeError(f"inv_freq must hold a multiple of 8 frequencies, at most head_dim / 2 = {D // 2}, got {half}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"positions must be int32 or int64 (got {positions.dtype})")
+    axes = 1 if positions.dim() == 1 else positions.size(0)
+    if positions.dim() not in (1, 2) or positions.size(-1) != T or not 1 <= axes <= 4:
+        raise RuntimeError(f"positions must be [tokens] or [axes, tokens] with up to four axes, got "
+                           f"{tuple(positions.shape)} for {T} tokens")
+    if sections is None:
+        if axes != 1:
+            raise RuntimeError("positions with several axes need sections")
+        ends = [half]
+    else:
+        ends, total = [], 0
+        for s in sections:
+            if s < 0:
+                raise RuntimeError(f"sections must not be negative, got {tuple(sections)}")
+            total += int(s)
+            ends.append(total)
+        if len(ends) != axes or total != half:
+            raise RuntimeError(f"sections {tuple(sections)} must give each of the {axes} axes its share of the {half} frequencies")
+    ends += [0] * (4 - axes)
+    kinds = set()
+    for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is None:
+            continue
+        if w.dim() != 1 or w.numel() != D:
+            raise RuntimeError(f"{n} must have {D} entries")
+        if w.dtype not in (q.dtype, torch.float32):
+            raise RuntimeError(f"{n} must be in the heads' dtype or fp32 (got {w.dtype})")
+        kinds.add(w.dtype)
+    if len(kinds) > 1:
+        raise RuntimeError("q_weight and k_weight must share a dtype")
+    weight_dtype = kinds.pop() if kinds else q.dtype
+    _require_cuda(q, "q")
+    for t, n in ((k, "k"), (q_weight, "q_weight"), (k_weight, "k_weight"), (positions, "positions"),
+                 (inv_freq, "inv_freq")):
+        if t is not None and t.device != q.device:
+            raise RuntimeError(f"{n} must be on q's device {q.device}, got {t.device}")
+    flags = (_NEIGHBOURS if interleaved else 0) | (_HADAMARD if hadamard else 0)
+    return D, 2 * half, flags, axes, ends, weight_dtype
+
+
+def _pack(q, k, tensors, D, R, flags, axes, ends, weight_dtype, positions, inv_freq, eps) -> bytes:
+    token, head = [0] * 6, [0] * 6
+    for i, t in enumerate(tensors):
+        token[i], head[i] = _head_strides(t)
+    return _HEADS.pack(q.size(0), *token, *head, q.size(1), k.size(1), D, R, axes, *ends,
+                       _DTYPE_CODE[q.dtype], _DTYPE_CODE[weight_dtype], 8 * positions.element_size(),
+                       8 * inv_freq.element_size(), flags, eps)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                 positions: torch.Tensor, inv_freq: torch.Tensor, *, eps: float = 1e-6,
+                 sections=None, interleaved: bool = False, hadamard: bool = False,
+                 inplace: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of each query and key head, rotation by the token's position and, with ``hadamard``,
+    ``H_D / sqrt(D)`` over the head, in one kernel; returns ``(q_out, k_out)``.
+
+    ``q`` ``[tokens, q_heads, D]`` and ``k`` ``[tokens, k_heads, D]`` in fp32, bf16 or fp16 may be views
+    into one packed projection output; ``D`` is a multiple of 16 up to 512.  Weights ``[D]`` (the heads'
+    dtype or fp32; ``None`` for ones).  Pair ``f`` turns by ``position * inv_freq[f]`` radians:
+    ``inv_freq`` (fp32 or fp64, a multiple of 8 frequencies) sets the rotary width ``R = 2 * len``, and
+    the values from ``R`` on are only normed.  The pairs are ``(i, i + R/2)``, or ``(2i, 2i + 1)`` with
+    ``interleaved``.  ``positions`` is ``[tokens]``, or ``[axes, tokens]`` with ``sections`` counting the
+    consecutive frequencies of each axis (time, height, width, ...).  Angles are formed in fp64, so far
+    positions keep their accuracy; the rest is fp32 with one rounding at the end.
+    ``inplace=True`` writes into ``q`` and ``k`` and returns them.
+    """
+    D, R, flags, axes, ends, wdt = _describe("qk_norm_rope", q, k, q_weight, k_weight, positions, inv_freq, eps,
+                                             sections, interleaved, hadamard)
+    _no_graph("qk_norm_rope", q, k, q_weight, k_weight)
+    if inplace and any(n > 1 and s == 0 for t in (q, k) for n, s in zip(t.shape, t.stride())):
+        raise RuntimeError("inplace needs heads that do not share memory (an expanded tensor was given)")
+    qs, ks = _readable(q), _readable(k)
+    if inplace:
+        qo, ko = qs, ks
+    else:
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if q.numel() or k.numel():
+        qw = None if q_weight is None else _dense16(q_weight)
+        kw = None if k_weight is None else _dense16(k_weight)
+        pos, freq = positions.contiguous(), inv_freq.contiguous()
+        lib = _lib.load()
+        with _on_device_of(q):
+            st = lib.mi_qk_norm_rope(qs.data_ptr(), ks.data_ptr(), _ptr(qw), _ptr(kw), pos.data_ptr(), freq.data_ptr(),
+                                     qo.data_ptr(), ko.data_ptr(),
+                                     _pack(qs, ks, (qs, ks, qo, ko), D, R, flags, axes, ends, wdt, pos, freq, eps),
+                                     _stream(q))
+        _lib.check(st, "qk_norm_rope")
+    if inplace:
+        if qs is not q:
+            q.copy_(qs)
+        if ks is not k:
+            k.copy_(ks)
+        return q, k
+    return qo, ko
+
+
+def qk_norm_rope_backward(q_grad: torch.Tensor, k_grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                          q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                          positions: torch.Tensor, inv_freq: torch.Tensor, *, eps: float = 1e-6,
+                          sections=None, interleaved: bool = False, hadamard: bool = False):
+    """Gradients of :func:`qk_norm_rope`: ``(dq, dk, dq_weight, dk_weight)`` from the gradients of its
+    outputs and its inputs ``q``, ``k`` (before the call, so not from an in-place one).  A weight that is
+    ``None`` has gradient ``None``; the others are in the weights' dtype, summed over all tokens and
+    heads in fp32 in a fixed order.
+    """
+    D, R, flags, axes, ends, wdt = _describe("qk_norm_rope_backward", q, k, q_weight, k_weight, positions, inv_freq,
+                                             eps, sections, interleaved, hadamard)
+    for g, t, n in ((q_grad, q, "q_grad"), (k_grad, k, "k_grad")):
+        if g.shape != t.shape or g.dtype != t.dtype:
+            raise RuntimeError(f"{n} must have the shape and dtype of {n[0]}: {tuple(t.shape)} {t.dtype}, got "
+                               f"{tuple(g.shape)} {g.dtype}")
+        if g.device != q.device:
+            raise RuntimeError(f"{n} must be on q's device {q.device}, got {g.device}")
+    dev = q.device
+    dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    dqw = None if q_weight is None else torch.empty(D, dtype=wdt, device=dev)
+    dkw = None if k_weight is None else torch.empty(D, dtype=wdt, device=dev)
+    qs, ks, qg, kg = _readable(q), _readable(k), _readable(q_grad), _readable(k_grad)
+    qw = None if q_weight is None else _dense16(q_weight)
+    kw = None if k_weight is None else _dense16(k_weight)
+    pos, freq = positions.contiguous(), inv_freq.contiguous()
+    lib = _lib.load()
+    workspace = None
+    if dqw is not None or dkw is not None:
+        workspace = torch.empty(lib.mi_qk_norm_rope_workspace(q.size(0), D), dtype=torch.uint8, device=dev)
+    with _on_device_of(q):
+        st = lib.mi_qk_norm_rope_backward(qs.data_ptr(), ks.data_ptr(), qg.data_ptr(), kg.data_ptr(), _ptr(qw), _ptr(kw),
+                                          pos.data_ptr(), freq.data_ptr(), dq.data_ptr(), dk.data_ptr(), _ptr(dqw), _ptr(dkw),
+                                          _ptr(workspace),
+                                          _pack(qs, ks, (qs, ks, qg, kg, dq, dk), D, R, flags, axes, ends, wdt, pos, freq, eps),
+                                          _stream(q))
+    _lib.check(st, "qk_norm_rope_backward")
+    return dq, dk, dqw, dkw

@@ -136,6 +136,61 @@ int mi_fp8_gemm_rowscale(const void* qa, const float* sa, const void* qb, const 
                          void* out, uint32_t T, uint32_t N, uint32_t K, void* stream);
 
 /*
+ * Query and key heads of a batch of tokens, for mi_qk_norm_rope and its backward pass.  Strides are in
+ * elements; base pointers are 16-byte aligned and strides multiples of 16 bytes; the values of a head
+ * are contiguous.  The stride arrays are indexed like the call's tensors: forward {q, k, q_out, k_out},
+ * backward {q, k, q_grad, k_grad, dq, dk}.
+ */
+typedef struct mi_heads {
+    uint64_t tokens;
+    uint64_t token_stride[6], head_stride[6];
+    uint32_t q_heads, k_heads;
+    uint32_t head_dim;        /* D: a multiple of 16, 16 ... 512                                     */
+    uint32_t rotary_dim;      /* R: a multiple of 16, 0 ... D; the first R values of a head turn     */
+    uint32_t axes;            /* position axes, 1 ... 4                                              */
+    uint32_t section_end[4];  /* frequencies [section_end[i-1], section_end[i]) take axis i; the last
+                                 of the `axes` entries is R / 2                                      */
+    int32_t dtype;            /* of q, k, the outputs and gradients                                  */
+    int32_t weight_dtype;     /* dtype, or MI_F32                                                    */
+    uint32_t position_bits;   /* 32 or 64: signed integers                                           */
+    uint32_t freq_bits;       /* 32 or 64: floats                                                    */
+    uint32_t flags;           /* MI_HEADS_...                                                        */
+    float eps;                /* >= 0                                                                */
+} mi_heads;
+#define MI_HEADS_NEIGHBOURS 1u /* the pairs are (2i, 2i+1); without it (i, i + R/2)                  */
+#define MI_HEADS_HADAMARD 2u   /* the heads leave rotated by H_D / sqrt(D); D a power of two         */
+
+/*
+ * Norm of each query and key head, position rotation and optional Hadamard rotation, in one pass:
+ *     n_i = x_i * (mean_j x_j^2 + eps)^-1/2 * weight_i
+ *     pair f of n turns by  positions[axis(f)][token] * inv_freq[f]  radians:
+ *     (a, b) -> (a cos - b sin, b cos + a sin);   values R ... D-1 stay
+ *     out = H_D n / sqrt(D)   with MI_HEADS_HADAMARD
+ * fp32 between the load and one rounding at the store; angles are formed and reduced in fp64.  The
+ * Hadamard rotation of queries and keys alike leaves their products as they are and spreads outlier
+ * channels before the keys are quantized.  No counterpart in the reference.
+ *   q_weight, k_weight : [D] or NULL (all ones).
+ *   positions          : [axes][tokens].      inv_freq : [R / 2].   (Not read when R = 0.)
+ *   q_out, k_out       : may be q, k (in place, same strides); no other overlap.
+ */
+int mi_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                    const void* positions, const void* inv_freq, void* q_out, void* k_out,
+                    const mi_heads* heads, void* stream);
+
+/*
+ * Gradients of mi_qk_norm_rope.  q, k are the forward pass's inputs, q_grad, k_grad the gradients of its
+ * outputs; dq, dk receive the gradients of q, k and overlap none of them.  dq_weight, dk_weight: [D] in
+ * weight_dtype, or NULL; they are sums over all tokens and heads, in a fixed order.
+ *   workspace : mi_qk_norm_rope_workspace(tokens, D) bytes, 16-byte aligned; not needed (NULL) when
+ *               both weight gradients are NULL.  Two kernels with weight gradients, else one.
+ */
+int mi_qk_norm_rope_backward(const void* q, const void* k, const void* q_grad, const void* k_grad,
+                             const void* q_weight, const void* k_weight, const void* positions,
+                             const void* inv_freq, void* dq, void* dk, void* dq_weight, void* dk_weight,
+                             void* workspace, const mi_heads* heads, void* stream);
+uint64_t mi_qk_norm_rope_workspace(uint64_t tokens, uint32_t head_dim);
+
+/*
  * One-wavefront MFMA layout check:  D[16,16] = A[16,Kk] * B[Kk,16]  with exactly one matrix-core
  * instruction, operands gathered under the register layout the kernels assume.
  * Mirrors the reference's test hook  test_mma_m16_n8_k16(x, y)  (csrc/test_frag.cu:8-62,
