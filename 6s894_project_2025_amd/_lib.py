@@ -21,6 +21,11 @@ SIGNATURES = {
     "mi_fused_ht_gemm": (_i, [_vp, _vp, _vp, _u32, _u32, _u32, _i, _i, _f, _vp]),
     "mi_rht_quant_fp8": (_i, [_vp, _vp, _vp, _vp, _vp, _u64, _u32, _f, _vp]),
     "mi_fp8_gemm_rowscale": (_i, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp]),
+    "mi_adapter_plan": (_i, [_vp, _i, _u64, _u32, _vp, _vp]),
+    "mi_adapter_plan_layout": (_i, [_u64, _u32, _vp]),
+    "mi_lora_add": (_i, [_vp] * 11),
+    "mi_lora_add_backward": (_i, [_vp] * 14),
+    "mi_lora_workspace": (_u64, [_vp, _i]),
     "mi_qk_norm_rope": (_i, [_vp] * 10),
     "mi_qk_norm_rope_backward": (_i, [_vp] * 15),
     "mi_qk_norm_rope_workspace": (_u64, [_u64, _u32]),

@@ -1,0 +1,46 @@
+// Layout of an adapter plan: a batch's tokens grouped by adapter, and the pieces of work that the
+// low-rank adapter kernels take from it.  One int32 buffer; the tables come first so that their
+// 16-byte entries are aligned.
+#pragma once
+#include "common.hpp"
+
+namespace mi {
+namespace adapters {
+
+constexpr uint32_t kTile = 64;        // tokens of one adapter that a workgroup takes together
+constexpr uint32_t kChunk = 512;      // tokens of one adapter behind one partial weight gradient
+constexpr uint32_t kMaxAdapters = 1024;
+// A grid has at most 65535 workgroups along its second axis, where chunks and parts of K or N are.
+constexpr uint64_t kMaxTokens = 1u << 24;
+constexpr uint32_t kMaxWidth = 1u << 22;
+
+struct Tile {  // positions [first, first + count) of the grouped order; adapter == n: tokens without one
+    int32_t adapter, first, count, unused;
+};
+struct Chunk {  // slot: row of partial sums, or -1 where the adapter has no other chunk
+    int32_t adapter, first, count, slot, tile, unused[3];
+};
+
+struct PlanLayout {
+    uint64_t max_tiles, max_chunks, max_slots;
+    uint64_t chunks, counts, slot_start, order, starts, size;  // offsets in int32; tiles are at 0
+
+    __host__ __device__ PlanLayout(uint64_t tokens, uint32_t n)
+    {
+        const uint64_t groups = tokens < n + 1ull ? tokens : n + 1ull;  // at most so many are not empty
+        max_tiles = tokens / kTile + groups;
+        max_chunks = tokens / kChunk + groups;
+        // only adapters with more than kChunk tokens have slots: at most tokens / kChunk of them, and
+        // ceil(c / kChunk) <= 2 c / kChunk for each
+        max_slots = 2u * (tokens / kChunk);
+        chunks = 4u * max_tiles;
+        counts = chunks + 8u * max_chunks;  // {tiles, chunks}
+        slot_start = counts + 2u;           // [n]
+        order = slot_start + n;             // [tokens]
+        starts = order + tokens;            // [n + 1]
+        size = starts + n + 1u;
+    }
+};
+
+}  // namespace adapters
+}  // namespace mi

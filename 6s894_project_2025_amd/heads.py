@@ -12,17 +12,11 @@ import struct
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _dense16, _is_pow2, _on_device_of, _require_cuda, _stream
+from .ops import _DTYPE_CODE, _dense16, _is_pow2, _no_graph, _on_device_of, _require_cuda, _stream
 
 _NEIGHBOURS, _HADAMARD = 1, 2
 _HEADS = struct.Struct("<Q6Q6Q4I" "I4I" "iiIII" "f4x")  # mi_heads
 _MAX_D = 512
-
-
-def _no_graph(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} records no autograd graph: call it under torch.no_grad() or inside a "
-                           f"torch.autograd.Function, and {name}_backward for the gradients")
 
 
 def _head_strides(t: torch.Tensor) -> tuple[int, int]:

@@ -57,6 +57,12 @@ def _dense16(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
+def _no_graph(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} records no autograd graph: call it under torch.no_grad() or inside a "
+                           f"torch.autograd.Function, and {name}_backward for the gradients")
+
+
 def hadamard_transform(x: torch.Tensor, scale: float | None = None, *, inplace: bool = False
                        ) -> torch.Tensor:
     """Walsh-Hadamard transform over the last dimension: ``y = scale * x @ H_n``.

@@ -136,6 +136,64 @@ int mi_fp8_gemm_rowscale(const void* qa, const float* sa, const void* qb, const 
                          void* out, uint32_t T, uint32_t N, uint32_t K, void* stream);
 
 /*
+ * Groups the tokens of a batch by the low-rank adapter they use: ids[t] in [0, n_adapters), anything
+ * else for a token without an adapter.  `plan` is an int32 buffer of layout[0] entries, 16-byte aligned,
+ * layout from mi_adapter_plan_layout for the same sizes; it stays valid for every call with this batch.
+ *   plan[layout[1] + i], i < tokens      : the tokens in grouped order (adapter by adapter, the tokens of
+ *                                          one in their own order, those without an adapter last)
+ *   plan[layout[2] + a], a <= n_adapters : first position of adapter a; [n_adapters] of the tokens without
+ * The rest is the kernels' own.  tokens <= 2^24, 1 <= n_adapters <= 1024, id_bits 32 or 64.
+ * One kernel; the result depends on the ids alone.  No counterpart in the reference.
+ */
+int mi_adapter_plan(const void* ids, int id_bits, uint64_t tokens, uint32_t n_adapters, int32_t* plan,
+                    void* stream);
+int mi_adapter_plan_layout(uint64_t tokens, uint32_t n_adapters, uint64_t layout[3]);
+
+/* Sizes of a batch with low-rank adapters.  Strides are row strides in elements, multiples of 16 bytes. */
+typedef struct mi_lora {
+    uint64_t tokens;      /* at most 2^24                                                   */
+    uint64_t x_stride;    /* of x                                                           */
+    uint64_t y_stride;    /* of y (forward), dy (backward)                                  */
+    uint64_t out_stride;  /* of out (forward), dx_in and dx (backward)                      */
+    uint32_t n_adapters;  /* 1 ... 1024, as in the plan                                     */
+    uint32_t rank;        /* a multiple of 8, 8 ... 128                                     */
+    uint32_t K, N;        /* input and output width: multiples of 8, 8 ... 2^22             */
+    int32_t dtype;        /* mi_dtype of every matrix                                       */
+} mi_lora;
+
+/*
+ * Low-rank adapters beside a shared projection, each token with its own:
+ *     u[t] = A[a] . x[t]      out[t] = y[t] + scales[a] * B[a] . u[t]      a = ids[t] of the plan
+ * and out[t] = y[t] for tokens without an adapter.  A [n_adapters][rank][K] and B [n_adapters][N][rank]
+ * are dense.  fp32 sums; u is kept to at least 16 significand bits between the products; out is rounded
+ * once.  An adapter of a smaller rank is padded with zeros.  No counterpart in the reference.
+ *   scales    : fp32 [n_adapters], or NULL for 1.
+ *   out       : may be y with the same stride (in place; other tokens' rows are then not touched); no
+ *               other overlap with any operand.
+ *   shrunk    : NULL, or fp32 [tokens][rank]: receives u (zeros for tokens without an adapter).
+ *   workspace : mi_lora_workspace(sizes, 0) bytes.
+ * All pointers 16-byte aligned (scales, shrunk: 4).  Two kernels.
+ */
+int mi_lora_add(const void* y, const void* x, const void* A, const void* B, const float* scales,
+                const int32_t* plan, void* out, float* shrunk, void* workspace, const mi_lora* sizes,
+                void* stream);
+
+/*
+ * Gradients of mi_lora_add (that of y is dy itself):
+ *     d[t] = scales[a] * B[a]^T . dy[t]        dx[t] = dx_in[t] + A[a]^T . d[t]
+ *     dA[a] = sum over its tokens of d[t] x[t]^T,   dB[a] = sum of scales[a] * dy[t] u[t]^T
+ * in a fixed order; dA, dB are shaped like A, B, zeros for adapters without tokens.
+ *   shrunk    : u from the forward pass, or NULL (it is computed again from x).
+ *   dx_in     : NULL for zeros, or added; may be dx (in place).
+ *   workspace : mi_lora_workspace(sizes, 1) bytes.  Outputs overlap no input but dx_in = dx.
+ */
+int mi_lora_add_backward(const void* dy, const void* x, const void* A, const void* B, const float* scales,
+                         const int32_t* plan, const float* shrunk, const void* dx_in, void* dx, void* dA,
+                         void* dB, void* workspace, const mi_lora* sizes, void* stream);
+/* Bytes of workspace, 16-byte aligned; 0 for sizes that the calls refuse. */
+uint64_t mi_lora_workspace(const mi_lora* sizes, int backward);
+
+/*
  * Query and key heads of a batch of tokens, for mi_qk_norm_rope and its backward pass.  Strides are in
  * elements; base pointers are 16-byte aligned and strides multiples of 16 bytes; the values of a head
  * are contiguous.  The stride arrays are indexed like the call's tensors: forward {q, k, q_out, k_out},

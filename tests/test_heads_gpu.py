@@ -440,11 +440,11 @@ def test_differentiable_inputs_are_refused_under_grad_mode(pkg):
         args[n] = args[n].float()
     # the device is checked first; the rule itself needs no device
     import importlib
-    heads = importlib.import_module(pkg.__name__ + ".heads")
+    ops = importlib.import_module(pkg.__name__ + ".ops")
     with pytest.raises(RuntimeError, match="no autograd graph"):
-        heads._no_graph("qk_norm_rope", args["q"], None)
+        ops._no_graph("qk_norm_rope", args["q"], None)
     with torch.no_grad():
-        heads._no_graph("qk_norm_rope", args["q"], None)
+        ops._no_graph("qk_norm_rope", args["q"], None)
 
 
 def test_lane_layout_covers_every_value_once():
