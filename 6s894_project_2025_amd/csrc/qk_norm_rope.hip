@@ -15,6 +15,10 @@
 // (Gray code): the lanes whose j differ in bit b alone are then l and l ^ (2^(b+1) - 1), which are
 // row mirrors and quad permutes, so the sums and the Hadamard butterflies across lanes cost no LDS.
 // Everything between the load and the one rounding at the store is fp32; angles are reduced in fp64.
+//
+// Work.  A wavefront takes 64 / 2^lg heads at a time (an item); a workgroup takes the query heads or the
+// key heads of a few tokens, so that one set of weights stays in registers, computes the tokens'
+// sines and cosines once into LDS, and requests two items ahead.
 #include <type_traits>
 
 #include "common.hpp"
@@ -23,37 +27,53 @@ namespace mi {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kMaxHalfRotary = 256;  // head_dim <= 512
+constexpr uint32_t kTableEntries = 1024;  // angles of a workgroup's tokens; a head has at most 256
 constexpr uint32_t kMaxPartials = 1024;   // workgroups of the backward pass, each with a row of partial sums
 
+struct Side {          // the queries, or the keys
+    const void* x;
+    const void* g;     // gradients of the outputs (backward)
+    void* y;           // outputs; gradients of x (backward)
+    const void* w;
+    uint64_t x_ts, x_hs, g_ts, g_hs, y_ts, y_hs;  // token and head strides, elements
+    uint32_t heads, per_block, blocks;            // tokens of a workgroup; workgroups
+};
+
 struct HeadsArgs {
-    const void* x[2];     // queries, keys
-    const void* g[2];     // gradients of the outputs (backward)
-    void* y[2];           // outputs; gradients of x (backward)
-    const void* w[2];
+    Side q, k;
     const void* positions;
     const void* freq;
-    float* partials;      // [workgroups][2][D] (backward)
+    float* partials;      // [workgroups][D] (backward)
     uint64_t tokens;
-    uint64_t x_ts[2], x_hs[2], g_ts[2], g_hs[2], y_ts[2], y_hs[2];  // token and head strides, elements
-    uint32_t heads[2];
     uint32_t D, R, lg;
     uint32_t section_end[3];
     float eps, out_scale;
     bool w_f32, pos64, freq64, neighbours, hadamard, mixed;
-    uint32_t tokens_per_block;  // 4: a wavefront per token; 1: the wavefronts share a token's heads
 };
 
+// A lane's unit as it comes from memory.
+template <class E> struct Raw { u32x4 v; };
+template <> struct Raw<float> { u32x4 v, w; };
+
 template <class E>
-__device__ __forceinline__ void load_unit(const E* p, float (&v)[8])
+__device__ __forceinline__ void fetch(Raw<E>& r, const E* p)
+{
+    r.v = *reinterpret_cast<const u32x4*>(p);
+    if constexpr (std::is_same<E, float>::value) r.w = *reinterpret_cast<const u32x4*>(p + 4);
+}
+
+template <class E>
+__device__ __forceinline__ void unpack(const Raw<E>& r, float (&v)[8])
 {
     if constexpr (std::is_same<E, float>::value) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+        for (int i = 0; i < 4; ++i) {
+            v[i] = __builtin_bit_cast(float, (uint32_t)r.v[i]);
+            v[4 + i] = __builtin_bit_cast(float, (uint32_t)r.w[i]);
+        }
     } else {
         typedef E V8 __attribute__((ext_vector_type(8)));
-        const V8 a = *reinterpret_cast<const V8*>(p);
+        const V8 a = __builtin_bit_cast(V8, r.v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
     }
@@ -84,7 +104,7 @@ __device__ __forceinline__ float mirror_lane(float v)
     if constexpr (STEP < 4) {
         constexpr int ctrl[4] = {0xB1, 0x1B, 0x141, 0x140};  // quad_perm 1,0,3,2 / 3,2,1,0; half row; row
         return __builtin_bit_cast(
-            float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl[STEP], 0xf, 0xf, false));
+            float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl[STEP], 0xf, 0xf, true));
     } else {
         return __shfl_xor(v, 31);
     }
@@ -100,20 +120,52 @@ __device__ __forceinline__ float lane_group_sum(float v, uint32_t lg)
     return v;
 }
 
+// One butterfly stage across lanes: with s = -1 in the lanes whose bit is set, the stage is
+// partner + s own; s (partner + s own) = own + s partner is one instruction per value instead of two.
+// The factor s stays in the lane and meets the partners' equal one in the other stages; what is left
+// at the end is one sign per lane, lane_sign().
 template <int STEP>
 __device__ __forceinline__ void lane_butterfly(float (&v)[2][8], uint32_t j)
 {
     const float s = (j >> STEP & 1u) ? -1.0f : 1.0f;
+    if constexpr (STEP < 4) {
+        // The compiler moves the partner's value into a register of its own first.  A register that a
+        // vector instruction has just written may be read across lanes two issue slots later.
+#define MI_STAGE8(u, CTRL)                                                                                            \
+    asm("s_nop 1\n\t"                                                                                                \
+        "v_fmac_f32_dpp %0, %0, %8 " CTRL " row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %1, %1, %8 " CTRL          \
+        " row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %2, %2, %8 " CTRL                                             \
+        " row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %3, %3, %8 " CTRL                                             \
+        " row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %4, %4, %8 " CTRL                                             \
+        " row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %5, %5, %8 " CTRL                                             \
+        " row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %6, %6, %8 " CTRL                                             \
+        " row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %7, %7, %8 " CTRL " row_mask:0xf bank_mask:0xf"               \
+        : "+v"(v[u][0]), "+v"(v[u][1]), "+v"(v[u][2]), "+v"(v[u][3]), "+v"(v[u][4]), "+v"(v[u][5]), "+v"(v[u][6]),     \
+          "+v"(v[u][7])                                                                                               \
+        : "v"(s))
+        if constexpr (STEP == 0) { MI_STAGE8(0, "quad_perm:[1,0,3,2]"); MI_STAGE8(1, "quad_perm:[1,0,3,2]"); }
+        if constexpr (STEP == 1) { MI_STAGE8(0, "quad_perm:[3,2,1,0]"); MI_STAGE8(1, "quad_perm:[3,2,1,0]"); }
+        if constexpr (STEP == 2) { MI_STAGE8(0, "row_half_mirror"); MI_STAGE8(1, "row_half_mirror"); }
+        if constexpr (STEP == 3) { MI_STAGE8(0, "row_mirror"); MI_STAGE8(1, "row_mirror"); }
+#undef MI_STAGE8
+    } else {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[u][i] = mirror_lane<STEP>(v[u][i]) + s * v[u][i];
+            for (int i = 0; i < 8; ++i) v[u][i] = __builtin_fmaf(mirror_lane<STEP>(v[u][i]), s, v[u][i]);
+    }
 }
+__device__ __forceinline__ float lane_sign(uint32_t j) { return __popc(j) & 1 ? -1.0f : 1.0f; }
 
-// Unnormalised H_D over the head: the index bits are 3 in a unit, 1 between the lane's units and lg
-// across lanes, and the stages commute.
+// lane_sign * unnormalised H_D over the head: the index bits are 3 in a unit, 1 between the lane's units
+// and lg across lanes, and the stages commute.
 __device__ __forceinline__ void head_butterflies(float (&v)[2][8], uint32_t j, uint32_t lg)
 {
+    if (lg > 0) lane_butterfly<0>(v, j);
+    if (lg > 1) lane_butterfly<1>(v, j);
+    if (lg > 2) lane_butterfly<2>(v, j);
+    if (lg > 3) lane_butterfly<3>(v, j);
+    if (lg > 4) lane_butterfly<4>(v, j);
 #pragma unroll
     for (int b = 1; b < 8; b <<= 1)
 #pragma unroll
@@ -131,21 +183,9 @@ __device__ __forceinline__ void head_butterflies(float (&v)[2][8], uint32_t j, u
         v[0][i] = p + q;
         v[1][i] = p - q;
     }
-    if (lg > 0) lane_butterfly<0>(v, j);
-    if (lg > 1) lane_butterfly<1>(v, j);
-    if (lg > 2) lane_butterfly<2>(v, j);
-    if (lg > 3) lane_butterfly<3>(v, j);
-    if (lg > 4) lane_butterfly<4>(v, j);
 }
 
-// Where unit u of a head is while it is laid out for a partial rotation of halves (0 < R < D).
-__device__ __forceinline__ void rotary_place(uint32_t u, uint32_t rl, uint32_t& j, uint32_t& slot)
-{
-    slot = u < rl ? 0u : u < 2u * rl ? 1u : u & 1u;
-    j = u < rl ? u : u < 2u * rl ? u - rl : u >> 1;
-}
-
-// From the layout for a partial rotation of halves to units 2j, 2j + 1 in lane j (and back, BACK).
+// From the layout for a partial rotation of halves (0 < R < D) to units 2j, 2j + 1 in lane j, or back.
 template <bool BACK>
 __device__ __forceinline__ void relayout(float (&v)[2][8], uint32_t lane, uint32_t j, uint32_t lg, uint32_t rl)
 {
@@ -154,15 +194,16 @@ __device__ __forceinline__ void relayout(float (&v)[2][8], uint32_t lane, uint32
 #pragma unroll
     for (uint32_t s = 0; s < 2; ++s) {
         uint32_t from_j, from_slot;
-        if (BACK) {  // unit that this lane's slot s holds in the rotary layout, found in the plain one
+        if (BACK) {  // the unit of slot s in the rotary layout, found in the plain one
             const uint32_t u = j < rl ? j + s * rl : 2u * j + s;
             from_j = u >> 1;
             from_slot = u & 1u;
         } else {
-            rotary_place(2u * j + s, rl, from_j, from_slot);
+            const uint32_t u = 2u * j + s;
+            from_slot = u < rl ? 0u : u < 2u * rl ? 1u : s;
+            from_j = u < rl ? u : u < 2u * rl ? u - rl : j;
         }
-        // lane of a unit: the inverse of the Gray code
-        uint32_t l = from_j;
+        uint32_t l = from_j;  // its lane: the inverse of the Gray code
         l ^= l >> 1;
         l ^= l >> 2;
         l ^= l >> 4;
@@ -180,24 +221,24 @@ __device__ __forceinline__ void relayout(float (&v)[2][8], uint32_t lane, uint32
 }
 
 // Rotation of a lane's eight pairs by its eight angles; DIR = -1 turns back.
-template <int DIR>
-__device__ __forceinline__ void rotate_pairs(float (&v)[2][8], const float (&c)[8], const float (&s)[8], bool neighbours)
+template <int DIR, bool NEIGHBOURS>
+__device__ __forceinline__ void rotate_pairs(float (&v)[2][8], const float2 (&cs)[8])
 {
-    if (neighbours) {
+    if (NEIGHBOURS) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float a = v[u][2 * i], b = v[u][2 * i + 1], cc = c[4 * u + i], ss = DIR * s[4 * u + i];
-                v[u][2 * i] = __builtin_fmaf(-b, ss, a * cc);
-                v[u][2 * i + 1] = __builtin_fmaf(a, ss, b * cc);
+                const float a = v[u][2 * i], b = v[u][2 * i + 1], c = cs[4 * u + i].x, s = DIR * cs[4 * u + i].y;
+                v[u][2 * i] = __builtin_fmaf(-b, s, a * c);
+                v[u][2 * i + 1] = __builtin_fmaf(a, s, b * c);
             }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float a = v[0][i], b = v[1][i], cc = c[i], ss = DIR * s[i];
-            v[0][i] = __builtin_fmaf(-b, ss, a * cc);
-            v[1][i] = __builtin_fmaf(a, ss, b * cc);
+            const float a = v[0][i], b = v[1][i], c = cs[i].x, s = DIR * cs[i].y;
+            v[0][i] = __builtin_fmaf(-b, s, a * c);
+            v[1][i] = __builtin_fmaf(a, s, b * c);
         }
     }
 }
@@ -222,232 +263,276 @@ __device__ __forceinline__ float2 turn(const HeadsArgs& a, uint64_t token, uint3
 struct LanePlace {
     uint32_t lane, group, groups, j, unit[2], plain[2];
     bool active, rotated;
-    __device__ __forceinline__ explicit LanePlace(const HeadsArgs& a)
+    __device__ __forceinline__ LanePlace(const HeadsArgs& a, uint32_t lg, bool neighbours)
     {
         lane = threadIdx.x & 63u;
-        const uint32_t l = lane & ((1u << a.lg) - 1u);
-        group = lane >> a.lg;
-        groups = 64u >> a.lg;
+        const uint32_t l = lane & ((1u << lg) - 1u);
+        group = lane >> lg;
+        groups = 64u >> lg;
         j = l ^ (l >> 1);
         active = j < a.D / 16u;
         const uint32_t rl = a.R / 16u;
         rotated = j < rl;
         plain[0] = 16u * j;
         plain[1] = 16u * j + 8u;
-        const bool halves = rotated && !a.neighbours;
+        const bool halves = rotated && !neighbours;
         unit[0] = halves ? 8u * j : plain[0];
         unit[1] = halves ? 8u * (j + rl) : plain[1];
     }
 };
 
-__device__ __forceinline__ void load_weight(const HeadsArgs& a, const LanePlace& p, int kind, float (&w)[2][8], int dtype)
+template <class E>
+__device__ __forceinline__ void load_weight(const HeadsArgs& a, const void* weight, const LanePlace& p, float (&w)[2][8])
 {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[u][i] = 1.0f;
-    if (!a.w[kind] || !p.active) return;
+    if (!weight || !p.active) return;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        if (dtype == MI_F32) load_unit(static_cast<const float*>(a.w[kind]) + p.unit[u], w[u]);
-        else if (dtype == MI_BF16) load_unit(static_cast<const __bf16*>(a.w[kind]) + p.unit[u], w[u]);
-        else load_unit(static_cast<const _Float16*>(a.w[kind]) + p.unit[u], w[u]);
+        if (a.w_f32) {
+            Raw<float> r;
+            fetch(r, static_cast<const float*>(weight) + p.unit[u]);
+            unpack(r, w[u]);
+        } else {
+            Raw<E> r;
+            fetch(r, static_cast<const E*>(weight) + p.unit[u]);
+            unpack(r, w[u]);
+        }
     }
 }
 
-template <class E> constexpr int dtype_of = MI_F32;
-template <> constexpr int dtype_of<__bf16> = MI_BF16;
-template <> constexpr int dtype_of<_Float16> = MI_F16;
+// The wavefront's items among `count` tokens of one kind: token and first head, four wavefronts in turn.
+struct Items {
+    uint32_t per_token, token, pass;
+    __device__ __forceinline__ Items(uint32_t heads, uint32_t groups, uint32_t wave)
+        : per_token((heads + groups - 1u) / groups), token(wave / per_token), pass(wave - wave / per_token * per_token)
+    {
+    }
+    __device__ __forceinline__ void next()
+    {
+        pass += 4u;
+        while (pass >= per_token) {
+            pass -= per_token;
+            ++token;
+        }
+    }
+};
 
-// Fills the cosine / sine table of the block's tokens.
-__device__ __forceinline__ void fill_turns(const HeadsArgs& a, uint64_t first, float2 (*table)[kMaxHalfRotary])
+// Fills the cosine / sine table of `count` tokens.
+__device__ __forceinline__ void fill_turns(const HeadsArgs& a, uint64_t first, uint32_t count, float2* table)
 {
     const uint32_t half = a.R / 2u;
-    for (uint32_t i = threadIdx.x; i < a.tokens_per_block * half; i += kThreads) {
-        const uint32_t t = i / half, f = i - t * half;
-        if (first + t < a.tokens) table[t][f] = turn(a, first + t, f);
+    for (uint32_t i = threadIdx.x; i < count * half; i += kThreads) {
+        const uint32_t t = i / half;
+        table[i] = turn(a, first + t, i - t * half);
     }
 }
 
-template <class E>
+// LG < 0: a.lg, any head size.  The common ones have kernels of their own (the branches on a run-time lg
+// keep the stages from overlapping).
+template <class E, int LG, bool NEIGHBOURS>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(HeadsArgs a)
 {
-    __shared__ float2 table[4][kMaxHalfRotary];
-    const LanePlace p(a);
-    const uint32_t wave = threadIdx.x >> 6;
-    const bool share = a.tokens_per_block == 1u;
-    const uint32_t rl = a.R / 16u;
-    const float inv_d = 1.0f / (float)a.D;
-    const int wdt = a.w_f32 ? MI_F32 : dtype_of<E>;
-    float w[2][2][8];
-    load_weight(a, p, 0, w[0], wdt);
-    load_weight(a, p, 1, w[1], wdt);
+    __shared__ float2 table[kTableEntries];
+    const uint32_t lg = LG < 0 ? a.lg : (uint32_t)LG;
+    const LanePlace p(a, lg, NEIGHBOURS);
+    const bool keys = blockIdx.x >= a.q.blocks;
+    const Side side = keys ? a.k : a.q;
+    const uint64_t first = (uint64_t)(blockIdx.x - (keys ? a.q.blocks : 0u)) * side.per_block;
+    const uint32_t count = (uint32_t)(a.tokens - first < side.per_block ? a.tokens - first : side.per_block);
+    const uint32_t heads = side.heads, half = a.R / 2u;
+    const bool hadamard = a.hadamard, mixed = !NEIGHBOURS && hadamard && a.mixed;
+    const E* x = static_cast<const E*>(side.x) + first * side.x_ts;
+    E* y = static_cast<E*>(side.y) + first * side.y_ts;
 
-    for (uint64_t first = (uint64_t)blockIdx.x * a.tokens_per_block; first < a.tokens;
-         first += (uint64_t)gridDim.x * a.tokens_per_block) {
-        __syncthreads();  // the table is still being read for the previous tokens
-        fill_turns(a, first, table);
-        __syncthreads();
-        const uint64_t token = first + (share ? 0u : wave);
-        if (token >= a.tokens) continue;  // no wavefront leaves: every one meets the barriers above
-        float c[8], s[8];
-        if (p.rotated) {
-            const float2* row = &table[share ? 0 : wave][8u * p.j];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { c[i] = row[i].x; s[i] = row[i].y; }
+    Raw<E> raw[2][2];
+    Items ahead(heads, p.groups, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), item = ahead;
+    auto request = [&](Raw<E> (&r)[2]) __attribute__((always_inline)) {
+        const uint32_t h = ahead.pass * p.groups + p.group;
+        if (ahead.token < count && p.active && h < heads) {
+            const E* row = x + ahead.token * side.x_ts + h * side.x_hs;
+            fetch(r[0], row + p.unit[0]);
+            fetch(r[1], row + p.unit[1]);
+        } else {
+            r[0] = r[1] = Raw<E>{};
         }
-        uint32_t pass = 0;
+        ahead.next();
+    };
+    request(raw[0]);
+    request(raw[1]);
+    float w[2][8];
+    load_weight<E>(a, side.w, p, w);
+    fill_turns(a, first, count, table);
+    __syncthreads();
+    const float inv_d = 1.0f / (float)a.D;
+    const float sign = hadamard ? lane_sign(p.j) * a.out_scale : 1.0f;
+
+    auto work = [&](Raw<E> (&r)[2]) __attribute__((always_inline)) {
+        float v[2][8];
+        unpack(r[0], v[0]);
+        unpack(r[1], v[1]);
+        request(r);
+        float ss = 0.0f;
 #pragma unroll
-        for (int kind = 0; kind < 2; ++kind) {
-            const E* x = static_cast<const E*>(a.x[kind]) + token * a.x_ts[kind];
-            E* y = static_cast<E*>(a.y[kind]) + token * a.y_ts[kind];
-            for (uint32_t h0 = 0; h0 < a.heads[kind]; h0 += p.groups, ++pass) {
-                if (share && (pass & 3u) != wave) continue;
-                const uint32_t h = h0 + p.group;
-                const bool here = p.active && h < a.heads[kind];
-                float v[2][8] = {};
-                if (here) {
-                    load_unit(x + h * a.x_hs[kind] + p.unit[0], v[0]);
-                    load_unit(x + h * a.x_hs[kind] + p.unit[1], v[1]);
-                }
-                float ss = 0.0f;
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(v[u][i], v[u][i], ss);
-                ss = lane_group_sum(ss, a.lg);
-                const float rho = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, inv_d, a.eps)) * a.out_scale;
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[u][i] = v[u][i] * rho * w[kind][u][i];
-                if (p.rotated) rotate_pairs<1>(v, c, s, a.neighbours);
-                if (a.hadamard) {
-                    if (a.mixed) relayout<false>(v, p.lane, p.j, a.lg, rl);
-                    head_butterflies(v, p.j, a.lg);
-                }
-                if (here) {
-                    const bool moved = a.hadamard && a.mixed;
-                    E* row = y + h * a.y_hs[kind];
-                    store_unit(row + (moved ? p.plain[0] : p.unit[0]), v[0]);
-                    store_unit(row + (moved ? p.plain[1] : p.unit[1]), v[1]);
-                }
+            for (int i = 0; i < 8; ++i) {
+                ss = __builtin_fmaf(v[u][i], v[u][i], ss);
+                v[u][i] *= w[u][i];
             }
+        if (p.rotated) {
+            float2 cs[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) cs[i] = table[item.token * half + 8u * p.j + i];
+            rotate_pairs<1, NEIGHBOURS>(v, cs);
         }
+        ss = lane_group_sum(ss, lg);
+        const float rho = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, inv_d, a.eps)) * sign;
+        if (hadamard) {
+            if (mixed) relayout<false>(v, p.lane, p.j, lg, a.R / 16u);
+            head_butterflies(v, p.j, lg);
+        }
+        const uint32_t h = item.pass * p.groups + p.group;
+        if (p.active && h < heads) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[u][i] *= rho;
+            E* row = y + item.token * side.y_ts + h * side.y_hs;
+            store_unit(row + (mixed ? p.plain[0] : p.unit[0]), v[0]);
+            store_unit(row + (mixed ? p.plain[1] : p.unit[1]), v[1]);
+        }
+        item.next();
+    };
+    while (item.token < count) {
+        work(raw[0]);
+        if (item.token >= count) break;
+        work(raw[1]);
     }
 }
 
-template <class E>
+template <class E, int LG, bool NEIGHBOURS>
 __global__ void __launch_bounds__(256) qk_norm_rope_backward_kernel(HeadsArgs a)
 {
-    __shared__ float2 table[4][kMaxHalfRotary];
-    const LanePlace p(a);
-    const uint32_t wave = threadIdx.x >> 6;
-    const bool share = a.tokens_per_block == 1u;
-    const uint32_t rl = a.R / 16u;
+    __shared__ float2 table[kTableEntries];
+    __shared__ float sums[4][512];
+    const uint32_t lg = LG < 0 ? a.lg : (uint32_t)LG;
+    const LanePlace p(a, lg, NEIGHBOURS);
+    const bool keys = blockIdx.x >= a.q.blocks;
+    const Side side = keys ? a.k : a.q;
+    const uint32_t block = blockIdx.x - (keys ? a.q.blocks : 0u), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t heads = side.heads, half = a.R / 2u;
+    const bool hadamard = a.hadamard, mixed = !NEIGHBOURS && hadamard && a.mixed;
+    const uint32_t g_unit[2] = {mixed ? p.plain[0] : p.unit[0], mixed ? p.plain[1] : p.unit[1]};
     const float inv_d = 1.0f / (float)a.D;
-    const int wdt = a.w_f32 ? MI_F32 : dtype_of<E>;
-    float w[2][2][8], dw[2][2][8] = {};
-    load_weight(a, p, 0, w[0], wdt);
-    load_weight(a, p, 1, w[1], wdt);
-    const bool moved = a.hadamard && a.mixed;
-    const uint32_t g_unit[2] = {moved ? p.plain[0] : p.unit[0], moved ? p.plain[1] : p.unit[1]};
+    const float sign = hadamard ? lane_sign(p.j) * a.out_scale : 1.0f;
+    float w[2][8], dw[2][8] = {};
+    load_weight<E>(a, side.w, p, w);
 
-    for (uint64_t first = (uint64_t)blockIdx.x * a.tokens_per_block; first < a.tokens;
-         first += (uint64_t)gridDim.x * a.tokens_per_block) {
+    for (uint64_t first = (uint64_t)block * side.per_block; first < a.tokens; first += (uint64_t)side.blocks * side.per_block) {
+        const uint32_t count = (uint32_t)(a.tokens - first < side.per_block ? a.tokens - first : side.per_block);
+        const E* x = static_cast<const E*>(side.x) + first * side.x_ts;
+        const E* g = static_cast<const E*>(side.g) + first * side.g_ts;
+        E* y = static_cast<E*>(side.y) + first * side.y_ts;
+        Raw<E> rx[2], rg[2];
+        Items ahead(heads, p.groups, wave), item = ahead;
+        auto request = [&]() __attribute__((always_inline)) {
+            const uint32_t h = ahead.pass * p.groups + p.group;
+            if (ahead.token < count && p.active && h < heads) {
+                const E* row = x + ahead.token * side.x_ts + h * side.x_hs;
+                const E* grad = g + ahead.token * side.g_ts + h * side.g_hs;
+                fetch(rx[0], row + p.unit[0]);
+                fetch(rx[1], row + p.unit[1]);
+                fetch(rg[0], grad + g_unit[0]);
+                fetch(rg[1], grad + g_unit[1]);
+            } else {
+                rx[0] = rx[1] = rg[0] = rg[1] = Raw<E>{};
+            }
+            ahead.next();
+        };
+        request();
+        __syncthreads();  // the table is still being read for the previous tokens
+        fill_turns(a, first, count, table);
         __syncthreads();
-        fill_turns(a, first, table);
-        __syncthreads();
-        const uint64_t token = first + (share ? 0u : wave);
-        if (token >= a.tokens) continue;
-        float c[8], s[8];
-        if (p.rotated) {
-            const float2* row = &table[share ? 0 : wave][8u * p.j];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { c[i] = row[i].x; s[i] = row[i].y; }
-        }
-        uint32_t pass = 0;
-#pragma unroll
-        for (int kind = 0; kind < 2; ++kind) {
-            const E* x = static_cast<const E*>(a.x[kind]) + token * a.x_ts[kind];
-            const E* g = static_cast<const E*>(a.g[kind]) + token * a.g_ts[kind];
-            E* y = static_cast<E*>(a.y[kind]) + token * a.y_ts[kind];
-            for (uint32_t h0 = 0; h0 < a.heads[kind]; h0 += p.groups, ++pass) {
-                if (share && (pass & 3u) != wave) continue;
-                const uint32_t h = h0 + p.group;
-                const bool here = p.active && h < a.heads[kind];
-                float v[2][8] = {}, d[2][8] = {};
-                if (here) {
-                    load_unit(x + h * a.x_hs[kind] + p.unit[0], v[0]);
-                    load_unit(x + h * a.x_hs[kind] + p.unit[1], v[1]);
-                    load_unit(g + h * a.g_hs[kind] + g_unit[0], d[0]);
-                    load_unit(g + h * a.g_hs[kind] + g_unit[1], d[1]);
-                }
-                if (a.hadamard) {
-                    head_butterflies(d, p.j, a.lg);
-                    if (a.mixed) relayout<true>(d, p.lane, p.j, a.lg, rl);
-                }
-                if (p.rotated) rotate_pairs<-1>(d, c, s, a.neighbours);
-                float ss = 0.0f, dot = 0.0f;
+        for (; item.token < count; item.next()) {
+            float v[2][8], d[2][8];
+            unpack(rx[0], v[0]);
+            unpack(rx[1], v[1]);
+            unpack(rg[0], d[0]);
+            unpack(rg[1], d[1]);
+            request();
+            if (hadamard) {
+                head_butterflies(d, p.j, lg);
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        d[u][i] *= a.out_scale;
-                        ss = __builtin_fmaf(v[u][i], v[u][i], ss);
-                        dot = __builtin_fmaf(d[u][i] * w[kind][u][i], v[u][i], dot);
-                    }
-                ss = lane_group_sum(ss, a.lg);
-                dot = lane_group_sum(dot, a.lg);
-                const float rho = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, inv_d, a.eps));
-                const float back = rho * rho * dot * inv_d;
-                float out[2][8];
+                    for (int i = 0; i < 8; ++i) d[u][i] *= sign;
+                if (mixed) relayout<true>(d, p.lane, p.j, lg, a.R / 16u);
+            }
+            if (p.rotated) {
+                float2 cs[8];
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int i = 0; i < 8; ++i) cs[i] = table[item.token * half + 8u * p.j + i];
+                rotate_pairs<-1, NEIGHBOURS>(d, cs);
+            }
+            float ss = 0.0f, dot = 0.0f, dn[2][8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        out[u][i] = rho * __builtin_fmaf(-back, v[u][i], d[u][i] * w[kind][u][i]);
-                        dw[kind][u][i] = __builtin_fmaf(d[u][i] * rho, v[u][i], dw[kind][u][i]);
-                    }
-                if (here) {
-                    E* row = y + h * a.y_hs[kind];
-                    store_unit(row + p.unit[0], out[0]);
-                    store_unit(row + p.unit[1], out[1]);
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    ss = __builtin_fmaf(v[u][i], v[u][i], ss);
+                    dn[u][i] = d[u][i] * v[u][i];
+                    d[u][i] *= w[u][i];
+                    dot = __builtin_fmaf(d[u][i], v[u][i], dot);
                 }
+            ss = lane_group_sum(ss, lg);
+            dot = lane_group_sum(dot, lg);
+            const float rho = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, inv_d, a.eps));
+            const float back = rho * rho * dot * inv_d;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    dw[u][i] = __builtin_fmaf(dn[u][i], rho, dw[u][i]);
+                    d[u][i] = rho * __builtin_fmaf(-back, v[u][i], d[u][i]);
+                }
+            const uint32_t h = item.pass * p.groups + p.group;
+            if (p.active && h < heads) {
+                E* row = y + item.token * side.y_ts + h * side.y_hs;
+                store_unit(row + p.unit[0], d[0]);
+                store_unit(row + p.unit[1], d[1]);
             }
         }
     }
 
     // Weight gradients of the workgroup: over the lane groups, then over the wavefronts, always in the
-    // same order.  Lanes without a head, or without a place in it, hold zeros.
-    __shared__ float sums[4][2][512];
+    // same order.  Lanes without a head hold zeros.
     if (!a.partials) return;
 #pragma unroll
-    for (int kind = 0; kind < 2; ++kind)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float t = dw[kind][u][i];
-                for (uint32_t step = 1u << a.lg; step < 64u; step <<= 1) t += __shfl_xor(t, (int)step);
-                if (p.active && p.group == 0) sums[wave][kind][p.unit[u] + i] = t;
-            }
+        for (int i = 0; i < 8; ++i) {
+            float t = dw[u][i];
+            for (uint32_t step = 1u << lg; step < 64u; step <<= 1) t += __shfl_xor(t, (int)step);
+            if (p.active && p.group == 0) sums[wave][p.unit[u] + i] = t;
+        }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 2u * a.D; i += kThreads) {
-        const uint32_t kind = i >= a.D, e = i - kind * a.D;
-        a.partials[(uint64_t)blockIdx.x * 2u * a.D + i] =
-            (sums[0][kind][e] + sums[1][kind][e]) + (sums[2][kind][e] + sums[3][kind][e]);
-    }
+    for (uint32_t i = threadIdx.x; i < a.D; i += kThreads)
+        a.partials[(uint64_t)blockIdx.x * a.D + i] = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
 }
 
-// Weight gradients: sums of the workgroups' rows, four columns per workgroup.
-__global__ void __launch_bounds__(256) weight_gradient_kernel(const float* partials, uint32_t rows, uint32_t D, void* dqw, void* dkw,
-                                                              int dtype)
+// Weight gradients: sums of the workgroups' rows, four columns per workgroup; blockIdx.y is the kind.
+__global__ void __launch_bounds__(256) weight_gradient_kernel(const float* partials, uint32_t rows_q, uint32_t rows_k, uint32_t D,
+                                                              void* dqw, void* dkw, int dtype)
 {
     __shared__ f32x4 part[256];
-    const uint32_t col = blockIdx.x * 4u;
+    const uint32_t col = blockIdx.x * 4u, r0 = blockIdx.y ? rows_q : 0u, r1 = r0 + (blockIdx.y ? rows_k : rows_q);
+    void* out = blockIdx.y ? dkw : dqw;
+    if (!out) return;
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t r = threadIdx.x; r < rows; r += 256u) t += *reinterpret_cast<const f32x4*>(partials + (uint64_t)r * 2u * D + col);
+    for (uint32_t r = r0 + threadIdx.x; r < r1; r += 256u) t += *reinterpret_cast<const f32x4*>(partials + (uint64_t)r * D + col);
     part[threadIdx.x] = t;
     __syncthreads();
     for (uint32_t half = 128u; half; half >>= 1) {
@@ -456,13 +541,10 @@ __global__ void __launch_bounds__(256) weight_gradient_kernel(const float* parti
     }
     if (threadIdx.x >= 4u) return;
     const uint32_t i = col + threadIdx.x;
-    void* out = i >= D ? dkw : dqw;
-    const uint32_t e = i >= D ? i - D : i;
     const float v = part[0][threadIdx.x];
-    if (!out) return;
-    if (dtype == MI_F32) static_cast<float*>(out)[e] = v;
-    else if (dtype == MI_BF16) static_cast<__bf16*>(out)[e] = (__bf16)v;
-    else static_cast<_Float16*>(out)[e] = (_Float16)v;
+    if (dtype == MI_F32) static_cast<float*>(out)[i] = v;
+    else if (dtype == MI_BF16) static_cast<__bf16*>(out)[i] = (__bf16)v;
+    else static_cast<_Float16*>(out)[i] = (_Float16)v;
 }
 
 // Checks a call and fills the kernel's arguments; `tensors` is 4 forward (x, y) and 6 backward (x, g, y).
@@ -487,8 +569,8 @@ int make_args(const mi_heads* d, const void* const* tensors, int count, const vo
     if (d->q_heads > 65536u || d->k_heads > 65536u || d->tokens >> 40) return MI_ERR_SHAPE;
     if (!(d->eps >= 0.0f)) return MI_ERR_SHAPE;
     a.tokens = d->tokens;
-    a.heads[0] = d->q_heads;
-    a.heads[1] = d->k_heads;
+    a.q.heads = d->q_heads;
+    a.k.heads = d->k_heads;
     a.D = d->head_dim;
     a.R = d->rotary_dim;
     a.lg = 0;
@@ -507,29 +589,81 @@ int make_args(const mi_heads* d, const void* const* tensors, int count, const vo
     const uint64_t unit = d->dtype == MI_F32 ? 4u : 8u;  // elements of 16 bytes
     if (d->tokens == 0 || d->q_heads + d->k_heads == 0) return MI_OK;
     for (int i = 0; i < count; ++i) {
-        if (a.heads[i & 1] == 0) continue;
+        if ((i & 1 ? d->k_heads : d->q_heads) == 0) continue;
         if (!tensors[i]) return MI_ERR_NULL;
         if (!aligned16(tensors[i]) || d->token_stride[i] % unit || d->head_stride[i] % unit) return MI_ERR_ALIGN;
     }
     if (a.R && (!positions || !inv_freq)) return MI_ERR_NULL;
     for (int kind = 0; kind < 2; ++kind) {
         const int out = count - 2 + kind;
-        a.x[kind] = tensors[kind];
-        a.x_ts[kind] = d->token_stride[kind];
-        a.x_hs[kind] = d->head_stride[kind];
-        a.g[kind] = count == 6 ? tensors[2 + kind] : nullptr;
-        a.g_ts[kind] = d->token_stride[2 + kind];
-        a.g_hs[kind] = d->head_stride[2 + kind];
-        a.y[kind] = const_cast<void*>(tensors[out]);
-        a.y_ts[kind] = d->token_stride[out];
-        a.y_hs[kind] = d->head_stride[out];
+        Side& side = kind ? a.k : a.q;
+        side.x = tensors[kind];
+        side.x_ts = d->token_stride[kind];
+        side.x_hs = d->head_stride[kind];
+        side.g = count == 6 ? tensors[2 + kind] : nullptr;
+        side.g_ts = d->token_stride[2 + kind];
+        side.g_hs = d->head_stride[2 + kind];
+        side.y = const_cast<void*>(tensors[out]);
+        side.y_ts = d->token_stride[out];
+        side.y_hs = d->head_stride[out];
     }
     return MI_OK;
 }
 
-// A wavefront per token once that gives every SIMD one (1024 tokens); fewer tokens than that are
-// spread over four wavefronts each.
-uint32_t tokens_per_block(uint64_t tokens) { return tokens >= 1024u ? 4u : 1u; }
+// Tokens per workgroup and workgroups of each kind.  Up to 8192 items (the wavefronts that the chip holds)
+// there is one for each wavefront; beyond, up to four, which keeps the table and the weights busy.
+void cut_work(HeadsArgs& a, uint64_t max_blocks)
+{
+    const uint32_t groups = 64u >> a.lg;
+    Side* const sides[2] = {&a.q, &a.k};
+    uint64_t items = 0, total = 0;
+    for (Side* s : sides) items += a.tokens * ((s->heads + groups - 1u) / groups);
+    const uint32_t per_wave = items <= 8192u ? 1u : items >= 4u * 8192u ? 4u : (uint32_t)(items / 8192u);
+    uint64_t wanted[2];
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t per_token = (sides[i]->heads + groups - 1u) / groups;
+        uint32_t n = per_token ? 4u * per_wave / per_token : 1u;
+        if (a.R && n > kTableEntries / (a.R / 2u)) n = kTableEntries / (a.R / 2u);
+        sides[i]->per_block = n ? n : 1u;
+        wanted[i] = per_token ? (a.tokens + sides[i]->per_block - 1u) / sides[i]->per_block : 0u;
+        total += wanted[i];
+    }
+    for (int i = 0; i < 2; ++i)  // in proportion where there are too many
+        sides[i]->blocks = (uint32_t)(total <= max_blocks ? wanted[i] : wanted[i] ? 1u + wanted[i] * (max_blocks - 2u) / total : 0u);
+}
+
+template <bool BACKWARD, class E, int LG, bool NEIGHBOURS>
+void launch(const HeadsArgs& a, hipStream_t s)
+{
+    const dim3 grid(a.q.blocks + a.k.blocks);
+    if (BACKWARD) hipLaunchKernelGGL((qk_norm_rope_backward_kernel<E, LG, NEIGHBOURS>), grid, dim3(kThreads), 0, s, a);
+    else hipLaunchKernelGGL((qk_norm_rope_kernel<E, LG, NEIGHBOURS>), grid, dim3(kThreads), 0, s, a);
+}
+
+template <bool BACKWARD, class E>
+int launch_for(const HeadsArgs& a, hipStream_t s)
+{
+    auto pick = [&](auto lg) {
+        constexpr int LG = decltype(lg)::value;
+        if (a.neighbours) launch<BACKWARD, E, LG, true>(a, s);
+        else launch<BACKWARD, E, LG, false>(a, s);
+    };
+    switch (a.lg) {
+        case 2: pick(std::integral_constant<int, 2>{}); break;   // heads of 48, 64
+        case 3: pick(std::integral_constant<int, 3>{}); break;   // 80 ... 128
+        case 4: pick(std::integral_constant<int, 4>{}); break;   // 144 ... 256
+        default: pick(std::integral_constant<int, -1>{}); break;
+    }
+    return launch_status();
+}
+
+template <bool BACKWARD>
+int launch_heads(const HeadsArgs& a, int dtype, hipStream_t s)
+{
+    if (dtype == MI_F32) return launch_for<BACKWARD, float>(a, s);
+    if (dtype == MI_BF16) return launch_for<BACKWARD, __bf16>(a, s);
+    return launch_for<BACKWARD, _Float16>(a, s);
+}
 
 }  // namespace
 }  // namespace mi
@@ -543,25 +677,17 @@ extern "C" int mi_qk_norm_rope(const void* q, const void* k, const void* q_weigh
     const int st = make_args(d, tensors, 4, positions, inv_freq, a);
     if (st != MI_OK) return st;
     if (d->tokens == 0 || d->q_heads + d->k_heads == 0) return MI_OK;
-    a.w[0] = q_weight;
-    a.w[1] = k_weight;
+    a.q.w = q_weight;
+    a.k.w = k_weight;
     if ((q_weight && !aligned16(q_weight)) || (k_weight && !aligned16(k_weight))) return MI_ERR_ALIGN;
-    a.tokens_per_block = tokens_per_block(d->tokens);
-    const uint64_t blocks = (d->tokens + a.tokens_per_block - 1u) / a.tokens_per_block;
-    const dim3 grid((uint32_t)(blocks < 2048u ? blocks : 2048u));
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    if (d->dtype == MI_F32) hipLaunchKernelGGL((qk_norm_rope_kernel<float>), grid, dim3(kThreads), 0, s, a);
-    else if (d->dtype == MI_BF16) hipLaunchKernelGGL((qk_norm_rope_kernel<__bf16>), grid, dim3(kThreads), 0, s, a);
-    else hipLaunchKernelGGL((qk_norm_rope_kernel<_Float16>), grid, dim3(kThreads), 0, s, a);
-    return launch_status();
+    cut_work(a, 1ull << 30);
+    return launch_heads<false>(a, d->dtype, static_cast<hipStream_t>(stream));
 }
 
 extern "C" uint64_t mi_qk_norm_rope_workspace(uint64_t tokens, uint32_t head_dim)
 {
     using namespace mi;
-    const uint32_t per = tokens_per_block(tokens);
-    const uint64_t blocks = tokens / per + (tokens % per != 0);
-    return (blocks < kMaxPartials ? blocks : kMaxPartials) * 2u * head_dim * sizeof(float);
+    return (tokens < kMaxPartials / 2u ? 2u * tokens : kMaxPartials) * head_dim * sizeof(float);
 }
 
 extern "C" int mi_qk_norm_rope_backward(const void* q, const void* k, const void* q_grad, const void* k_grad, const void* q_weight,
@@ -573,29 +699,23 @@ extern "C" int mi_qk_norm_rope_backward(const void* q, const void* k, const void
     const void* tensors[6] = {q, k, q_grad, k_grad, dq, dk};
     const int st = make_args(d, tensors, 6, positions, inv_freq, a);
     if (st != MI_OK) return st;
-    a.w[0] = q_weight;
-    a.w[1] = k_weight;
+    a.q.w = q_weight;
+    a.k.w = k_weight;
     if ((q_weight && !aligned16(q_weight)) || (k_weight && !aligned16(k_weight))) return MI_ERR_ALIGN;
     const bool any = d->tokens != 0 && d->q_heads + d->k_heads != 0;
     const bool weights = dq_weight || dk_weight;
     if (weights && any && !workspace) return MI_ERR_NULL;
     if (weights && any && !aligned16(workspace)) return MI_ERR_ALIGN;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    uint32_t grid = 0;
     if (any) {
         a.partials = weights ? static_cast<float*>(workspace) : nullptr;
-        a.tokens_per_block = tokens_per_block(d->tokens);
-        const uint64_t blocks = (d->tokens + a.tokens_per_block - 1u) / a.tokens_per_block;
-        grid = (uint32_t)(blocks < kMaxPartials ? blocks : kMaxPartials);
-        if (d->dtype == MI_F32) hipLaunchKernelGGL((qk_norm_rope_backward_kernel<float>), dim3(grid), dim3(kThreads), 0, s, a);
-        else if (d->dtype == MI_BF16) hipLaunchKernelGGL((qk_norm_rope_backward_kernel<__bf16>), dim3(grid), dim3(kThreads), 0, s, a);
-        else hipLaunchKernelGGL((qk_norm_rope_backward_kernel<_Float16>), dim3(grid), dim3(kThreads), 0, s, a);
-        const int launched = launch_status();
+        cut_work(a, kMaxPartials);
+        const int launched = launch_heads<true>(a, d->dtype, s);
         if (launched != MI_OK) return launched;
     }
     if (weights) {
-        hipLaunchKernelGGL(weight_gradient_kernel, dim3(a.D / 2u), dim3(256), 0, s, static_cast<const float*>(workspace), grid, a.D,
-                           dq_weight, dk_weight, d->weight_dtype);
+        hipLaunchKernelGGL(weight_gradient_kernel, dim3(a.D / 4u, 2), dim3(256), 0, s, static_cast<const float*>(workspace), a.q.blocks,
+                           a.k.blocks, a.D, dq_weight, dk_weight, d->weight_dtype);
         return launch_status();
     }
     return MI_OK;

@@ -428,7 +428,7 @@ def test_c_entry_refusals(pkg):
     assert call(desc(), w=p + 2) == ALIGN and back(desc(), ws=None) == NULL and back(desc(), ws=p + 4) == ALIGN
     assert call(desc(T=0), q=None) == 0 and call(desc(Hq=0, Hk=0), q=None) == 0
     assert lib.mi_qk_norm_rope_workspace(0, 64) == 0
-    assert lib.mi_qk_norm_rope_workspace(1, 64) == 2 * 64 * 4
+    assert lib.mi_qk_norm_rope_workspace(1, 64) == 2 * 64 * 4  # a row for the queries, a row for the keys
     sizes = [lib.mi_qk_norm_rope_workspace(t, 64) for t in (1023, 1024, 4096, 1 << 39)]
     assert all(s <= 1024 * 2 * 64 * 4 for s in sizes)
 
