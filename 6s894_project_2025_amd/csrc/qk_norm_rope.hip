@@ -16,9 +16,11 @@
 // row mirrors and quad permutes, so the sums and the Hadamard butterflies across lanes cost no LDS.
 // Everything between the load and the one rounding at the store is fp32; angles are reduced in fp64.
 //
-// Work.  A wavefront takes 64 / 2^lg heads at a time (an item); a workgroup takes the query heads or the
-// key heads of a few tokens, so that one set of weights stays in registers, computes the tokens'
-// sines and cosines once into LDS, and requests two items ahead.
+// Work.  A wavefront takes 64 / 2^lg heads at a time (an item).  Workgroups are for the query heads or for
+// the key heads, so that one set of weights stays in registers; a unit of work is a token's heads, or a part of
+// them where there are few tokens.  A wavefront computes the sines and cosines of its token once (one angle
+// per lane, exchanged through LDS that no other wavefront uses, so there is no barrier) and keeps requests
+// for the next items, of its next tokens too, in flight.
 #include <type_traits>
 
 #include "common.hpp"
@@ -27,8 +29,9 @@ namespace mi {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kTableEntries = 1024;  // angles of a workgroup's tokens; a head has at most 256
-constexpr uint32_t kMaxPartials = 1024;   // workgroups of the backward pass, each with a row of partial sums
+constexpr uint32_t kMaxHalfRotary = 256;  // angles of a token, head_dim <= 512
+constexpr uint32_t kMaxBlocks = 2048;     // eight workgroups per compute unit
+constexpr uint32_t kMaxPartials = 512;    // of the backward pass: two per compute unit; each has a row of partial sums
 
 struct Side {          // the queries, or the keys
     const void* x;
@@ -36,7 +39,7 @@ struct Side {          // the queries, or the keys
     void* y;           // outputs; gradients of x (backward)
     const void* w;
     uint64_t x_ts, x_hs, g_ts, g_hs, y_ts, y_hs;  // token and head strides, elements
-    uint32_t heads, per_block, blocks;            // tokens of a workgroup; workgroups
+    uint32_t heads, lg_parts, blocks;             // wavefronts that share a token's heads; workgroups
 };
 
 struct HeadsArgs {
@@ -79,6 +82,17 @@ __device__ __forceinline__ void unpack(const Raw<E>& r, float (&v)[8])
     }
 }
 
+// Both units of a lane.  The values are pinned here, before the next request takes the registers they came in.
+template <class E>
+__device__ __forceinline__ void unpack_units(const Raw<E> (&r)[2], float (&v)[2][8])
+{
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        unpack(r[u], v[u]);
+        asm volatile("" : "+v"(v[u][0]), "+v"(v[u][1]), "+v"(v[u][2]), "+v"(v[u][3]), "+v"(v[u][4]), "+v"(v[u][5]), "+v"(v[u][6]), "+v"(v[u][7]));
+    }
+}
+
 template <class E>
 __device__ __forceinline__ void store_unit(E* p, const float (&v)[8])
 {
@@ -93,7 +107,7 @@ __device__ __forceinline__ void store_unit(E* p, const float (&v)[8])
         V8 a;
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[i] = (E)v[i];
-        *reinterpret_cast<V8*>(p) = a;
+        __builtin_nontemporal_store(a, reinterpret_cast<V8*>(p));
     }
 }
 
@@ -243,23 +257,55 @@ __device__ __forceinline__ void rotate_pairs(float (&v)[2][8], const float2 (&cs
     }
 }
 
-// cos and sin of position * inv_freq.  The product and its reduction to a part of a turn are fp64: an
-// fp32 angle of position 10^5 would be off by 4e-3.
-__device__ __forceinline__ float2 turn(const HeadsArgs& a, uint64_t token, uint32_t f)
-{
-    const uint32_t axis = (f >= a.section_end[0]) + (f >= a.section_end[1]) + (f >= a.section_end[2]);
-    const uint64_t at = axis * a.tokens + token;
-    const double pos = a.pos64 ? (double)static_cast<const int64_t*>(a.positions)[at]
-                               : (double)static_cast<const int32_t*>(a.positions)[at];
-    const double freq = a.freq64 ? static_cast<const double*>(a.freq)[f] : (double)static_cast<const float*>(a.freq)[f];
-    const double turns = pos * freq * 0.15915494309189533577;
-    const float r = (float)(turns - __builtin_rint(turns));
-    float2 cs;
-    sincospif(2.0f * r, &cs.y, &cs.x);
-    return cs;
-}
+// A lane's angles: frequencies lane, lane + 64, ... (FREQS of them) of the wavefront's token.  The product of position and
+// frequency and its reduction to a part of a turn are fp64: an fp32 angle of position 10^5 would be
+// off by 4e-3.
+template <uint32_t FREQS, uint32_t I = 0>
+struct Turns {
+    double freq = 0.0;           // turns per position
+    uint64_t at = 0;             // of the lane's axis in positions
+    uint32_t low = 0, high = 0;  // the position as it comes from memory
+    Turns<FREQS, I + 1> rest;
 
-// The lane's place in its head and in the wavefront.
+    __device__ __forceinline__ explicit Turns(const HeadsArgs& a) : rest(a)
+    {
+        const uint32_t f = (threadIdx.x & 63u) + 64u * I;
+        if (f < a.R / 2u) {
+            freq = a.freq64 ? static_cast<const double*>(a.freq)[f] : (double)static_cast<const float*>(a.freq)[f];
+            freq *= 0.15915494309189533577;
+            at = ((f >= a.section_end[0]) + (f >= a.section_end[1]) + (f >= a.section_end[2])) * a.tokens;
+        }
+    }
+    __device__ __forceinline__ void request(const HeadsArgs& a, uint64_t token)  // not without frequencies
+    {
+        const uint32_t* words = static_cast<const uint32_t*>(a.positions) + ((at + token) << a.pos64);
+        low = words[0];
+        high = words[a.pos64];  // not used with 32 bits; no branch, so that the loads can be counted
+        rest.request(a, token);
+    }
+    __device__ __forceinline__ void fill(const HeadsArgs& a, float2* table)
+    {
+        const uint32_t f = (threadIdx.x & 63u) + 64u * I;
+        const double pos = a.pos64 ? (double)(int64_t)((uint64_t)high << 32 | low) : (double)(int32_t)low;
+        const double turns = pos * freq;
+        const float r = (float)(turns - __builtin_rint(turns));
+        float2 cs;
+        sincospif(2.0f * r, &cs.y, &cs.x);
+        if (f < a.R / 2u) table[f] = cs;
+        rest.fill(a, table);
+    }
+};
+template <uint32_t FREQS>
+struct Turns<FREQS, FREQS> {
+    __device__ __forceinline__ explicit Turns(const HeadsArgs&) {}
+    __device__ __forceinline__ void request(const HeadsArgs&, uint64_t) {}
+    __device__ __forceinline__ void fill(const HeadsArgs&, float2*) {}
+};
+
+// The lane's place in its head and in the wavefront.  A lane without a part of the head (head_dim / 16 is not a
+// power of two) does what the first lane does, and its sums count as zero; lanes behind the last head do
+// what the last head's lanes do.  They store the same values to the same place, so every load and store is
+// made by all lanes: behind a branch, a wait for one request would be a wait for all.
 struct LanePlace {
     uint32_t lane, group, groups, j, unit[2], plain[2];
     bool active, rotated;
@@ -271,6 +317,7 @@ struct LanePlace {
         groups = 64u >> lg;
         j = l ^ (l >> 1);
         active = j < a.D / 16u;
+        if (!active) j = 0;
         const uint32_t rl = a.R / 16u;
         rotated = j < rl;
         plain[0] = 16u * j;
@@ -278,6 +325,11 @@ struct LanePlace {
         const bool halves = rotated && !neighbours;
         unit[0] = halves ? 8u * j : plain[0];
         unit[1] = halves ? 8u * (j + rl) : plain[1];
+    }
+    __device__ __forceinline__ uint64_t head(uint32_t pass, uint32_t heads) const
+    {
+        const uint32_t h = pass * groups + group;
+        return h < heads ? h : heads - 1u;
     }
 };
 
@@ -288,7 +340,7 @@ __device__ __forceinline__ void load_weight(const HeadsArgs& a, const void* weig
     for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[u][i] = 1.0f;
-    if (!weight || !p.active) return;
+    if (!weight) return;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         if (a.w_f32) {
@@ -303,166 +355,171 @@ __device__ __forceinline__ void load_weight(const HeadsArgs& a, const void* weig
     }
 }
 
-// The wavefront's items among `count` tokens of one kind: token and first head, four wavefronts in turn.
-struct Items {
-    uint32_t per_token, token, pass;
-    __device__ __forceinline__ Items(uint32_t heads, uint32_t groups, uint32_t wave)
-        : per_token((heads + groups - 1u) / groups), token(wave / per_token), pass(wave - wave / per_token * per_token)
+// Waits for every load so far (s_waitcnt vmcnt(0)).  Inside the loops each wait then stands behind the same
+// loads and stores on every path, and the compiler lets the later ones stay in flight; without it the way
+// in, which may have none behind it, would have every item wait for the item before it to be stored.
+__device__ __forceinline__ void first_loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
+// A wavefront's way through its items: units (a token's heads, every 2^lg_parts-th group of them) in steps of
+// all the side's wavefronts.
+struct Cursor {
+    uint64_t unit, stride;
+    uint32_t lg_parts, per_token, pass;
+    __device__ __forceinline__ Cursor(const Side& s, uint32_t groups, uint32_t wavefront)
+        : unit(wavefront), stride(4u * s.blocks), lg_parts(s.lg_parts), per_token((s.heads + groups - 1u) / groups)
     {
+        pass = (uint32_t)unit & ((1u << lg_parts) - 1u);
     }
-    __device__ __forceinline__ void next()
+    __device__ __forceinline__ uint64_t token() const { return unit >> lg_parts; }
+    // true when the next item is another token's
+    __device__ __forceinline__ bool next()
     {
-        pass += 4u;
-        while (pass >= per_token) {
-            pass -= per_token;
-            ++token;
-        }
+        pass += 1u << lg_parts;
+        if (pass < per_token) return false;
+        unit += stride;
+        pass = (uint32_t)unit & ((1u << lg_parts) - 1u);
+        return true;
     }
 };
-
-// Fills the cosine / sine table of `count` tokens.
-__device__ __forceinline__ void fill_turns(const HeadsArgs& a, uint64_t first, uint32_t count, float2* table)
-{
-    const uint32_t half = a.R / 2u;
-    for (uint32_t i = threadIdx.x; i < count * half; i += kThreads) {
-        const uint32_t t = i / half;
-        table[i] = turn(a, first + t, i - t * half);
-    }
-}
 
 // LG < 0: a.lg, any head size.  The common ones have kernels of their own (the branches on a run-time lg
 // keep the stages from overlapping).
 template <class E, int LG, bool NEIGHBOURS>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(HeadsArgs a)
 {
-    __shared__ float2 table[kTableEntries];
+    __shared__ float2 tables[4][kMaxHalfRotary];
     const uint32_t lg = LG < 0 ? a.lg : (uint32_t)LG;
     const LanePlace p(a, lg, NEIGHBOURS);
     const bool keys = blockIdx.x >= a.q.blocks;
     const Side side = keys ? a.k : a.q;
-    const uint64_t first = (uint64_t)(blockIdx.x - (keys ? a.q.blocks : 0u)) * side.per_block;
-    const uint32_t count = (uint32_t)(a.tokens - first < side.per_block ? a.tokens - first : side.per_block);
-    const uint32_t heads = side.heads, half = a.R / 2u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t heads = side.heads;
     const bool hadamard = a.hadamard, mixed = !NEIGHBOURS && hadamard && a.mixed;
-    const E* x = static_cast<const E*>(side.x) + first * side.x_ts;
-    E* y = static_cast<E*>(side.y) + first * side.y_ts;
+    const E* x = static_cast<const E*>(side.x);
+    E* y = static_cast<E*>(side.y);
+    float2* table = tables[wave];
 
-    Raw<E> raw[2][2];
-    Items ahead(heads, p.groups, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), item = ahead;
-    auto request = [&](Raw<E> (&r)[2]) __attribute__((always_inline)) {
-        const uint32_t h = ahead.pass * p.groups + p.group;
-        if (ahead.token < count && p.active && h < heads) {
-            const E* row = x + ahead.token * side.x_ts + h * side.x_hs;
-            fetch(r[0], row + p.unit[0]);
-            fetch(r[1], row + p.unit[1]);
-        } else {
-            r[0] = r[1] = Raw<E>{};
-        }
+    Raw<E> raw[2];
+    Cursor ahead(side, p.groups, 4u * (blockIdx.x - (keys ? a.q.blocks : 0u)) + wave), item = ahead;
+    auto request = [&]() __attribute__((always_inline)) {
+        // behind the last item: the first token's row, which the cache holds
+        const uint64_t token = ahead.token() < a.tokens ? ahead.token() : 0u;
+        const E* row = x + token * side.x_ts + p.head(ahead.pass, heads) * side.x_hs;
+        fetch(raw[0], row + p.unit[0]);
+        fetch(raw[1], row + p.unit[1]);
         ahead.next();
     };
-    request(raw[0]);
-    request(raw[1]);
+    if (item.token() >= a.tokens) return;
+    request();
+    Turns<LG < 0 ? 4 : LG < 4 ? 1 : 2> turns(a);
+    if (a.R) turns.request(a, item.token());
     float w[2][8];
     load_weight<E>(a, side.w, p, w);
-    fill_turns(a, first, count, table);
-    __syncthreads();
     const float inv_d = 1.0f / (float)a.D;
     const float sign = hadamard ? lane_sign(p.j) * a.out_scale : 1.0f;
+    float2 cs[8];
+    first_loads_done();
 
-    auto work = [&](Raw<E> (&r)[2]) __attribute__((always_inline)) {
-        float v[2][8];
-        unpack(r[0], v[0]);
-        unpack(r[1], v[1]);
-        request(r);
-        float ss = 0.0f;
+    while (item.token() < a.tokens) {
+        __builtin_amdgcn_wave_barrier();
+        turns.fill(a, table);
+        __builtin_amdgcn_wave_barrier();
+        if (p.rotated)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+            for (int i = 0; i < 8; ++i) cs[i] = table[8u * p.j + i];
+        const uint64_t next = (item.unit + item.stride) >> item.lg_parts;
+        if (a.R) turns.request(a, next < a.tokens ? next : 0u);
+        do {
+            float v[2][8];
+            unpack_units(raw, v);
+            request();
+            float ss = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                ss = __builtin_fmaf(v[u][i], v[u][i], ss);
-                v[u][i] *= w[u][i];
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    ss = __builtin_fmaf(v[u][i], v[u][i], ss);
+                    v[u][i] *= w[u][i];
+                }
+            if (p.rotated) rotate_pairs<1, NEIGHBOURS>(v, cs);
+            ss = lane_group_sum(p.active ? ss : 0.0f, lg);
+            const float rho = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, inv_d, a.eps)) * sign;
+            if (hadamard) {
+                if (mixed) relayout<false>(v, p.lane, p.j, lg, a.R / 16u);
+                head_butterflies(v, p.j, lg);
             }
-        if (p.rotated) {
-            float2 cs[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) cs[i] = table[item.token * half + 8u * p.j + i];
-            rotate_pairs<1, NEIGHBOURS>(v, cs);
-        }
-        ss = lane_group_sum(ss, lg);
-        const float rho = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, inv_d, a.eps)) * sign;
-        if (hadamard) {
-            if (mixed) relayout<false>(v, p.lane, p.j, lg, a.R / 16u);
-            head_butterflies(v, p.j, lg);
-        }
-        const uint32_t h = item.pass * p.groups + p.group;
-        if (p.active && h < heads) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[u][i] *= rho;
-            E* row = y + item.token * side.y_ts + h * side.y_hs;
+            E* row = y + item.token() * side.y_ts + p.head(item.pass, heads) * side.y_hs;
             store_unit(row + (mixed ? p.plain[0] : p.unit[0]), v[0]);
             store_unit(row + (mixed ? p.plain[1] : p.unit[1]), v[1]);
-        }
-        item.next();
-    };
-    while (item.token < count) {
-        work(raw[0]);
-        if (item.token >= count) break;
-        work(raw[1]);
+        } while (!item.next());
     }
 }
 
 template <class E, int LG, bool NEIGHBOURS>
 __global__ void __launch_bounds__(256) qk_norm_rope_backward_kernel(HeadsArgs a)
 {
-    __shared__ float2 table[kTableEntries];
+    __shared__ float2 tables[4][kMaxHalfRotary];
     __shared__ float sums[4][512];
     const uint32_t lg = LG < 0 ? a.lg : (uint32_t)LG;
     const LanePlace p(a, lg, NEIGHBOURS);
     const bool keys = blockIdx.x >= a.q.blocks;
     const Side side = keys ? a.k : a.q;
-    const uint32_t block = blockIdx.x - (keys ? a.q.blocks : 0u), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t heads = side.heads, half = a.R / 2u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t heads = side.heads;
     const bool hadamard = a.hadamard, mixed = !NEIGHBOURS && hadamard && a.mixed;
     const uint32_t g_unit[2] = {mixed ? p.plain[0] : p.unit[0], mixed ? p.plain[1] : p.unit[1]};
+    const E* x = static_cast<const E*>(side.x);
+    const E* g = static_cast<const E*>(side.g);
+    E* y = static_cast<E*>(side.y);
+    float2* table = tables[wave];
     const float inv_d = 1.0f / (float)a.D;
     const float sign = hadamard ? lane_sign(p.j) * a.out_scale : 1.0f;
+
+    Raw<E> rx[2], rg[2];
+    Cursor ahead(side, p.groups, 4u * (blockIdx.x - (keys ? a.q.blocks : 0u)) + wave), item = ahead;
+    auto request = [&]() __attribute__((always_inline)) {
+        const uint64_t token = ahead.token() < a.tokens ? ahead.token() : 0u, h = p.head(ahead.pass, heads);
+        const E* row = x + token * side.x_ts + h * side.x_hs;
+        const E* grad = g + token * side.g_ts + h * side.g_hs;
+        fetch(rx[0], row + p.unit[0]);
+        fetch(rx[1], row + p.unit[1]);
+        fetch(rg[0], grad + g_unit[0]);
+        fetch(rg[1], grad + g_unit[1]);
+        ahead.next();
+    };
+    request();
+    Turns<LG < 0 ? 4 : LG < 4 ? 1 : 2> turns(a);
+    if (a.R) turns.request(a, item.token() < a.tokens ? item.token() : 0u);
     float w[2][8], dw[2][8] = {};
     load_weight<E>(a, side.w, p, w);
+    float2 cs[8];
+    first_loads_done();
 
-    for (uint64_t first = (uint64_t)block * side.per_block; first < a.tokens; first += (uint64_t)side.blocks * side.per_block) {
-        const uint32_t count = (uint32_t)(a.tokens - first < side.per_block ? a.tokens - first : side.per_block);
-        const E* x = static_cast<const E*>(side.x) + first * side.x_ts;
-        const E* g = static_cast<const E*>(side.g) + first * side.g_ts;
-        E* y = static_cast<E*>(side.y) + first * side.y_ts;
-        Raw<E> rx[2], rg[2];
-        Items ahead(heads, p.groups, wave), item = ahead;
-        auto request = [&]() __attribute__((always_inline)) {
-            const uint32_t h = ahead.pass * p.groups + p.group;
-            if (ahead.token < count && p.active && h < heads) {
-                const E* row = x + ahead.token * side.x_ts + h * side.x_hs;
-                const E* grad = g + ahead.token * side.g_ts + h * side.g_hs;
-                fetch(rx[0], row + p.unit[0]);
-                fetch(rx[1], row + p.unit[1]);
-                fetch(rg[0], grad + g_unit[0]);
-                fetch(rg[1], grad + g_unit[1]);
-            } else {
-                rx[0] = rx[1] = rg[0] = rg[1] = Raw<E>{};
-            }
-            ahead.next();
-        };
-        request();
-        __syncthreads();  // the table is still being read for the previous tokens
-        fill_turns(a, first, count, table);
-        __syncthreads();
-        for (; item.token < count; item.next()) {
+    while (item.token() < a.tokens) {
+        __builtin_amdgcn_wave_barrier();
+        turns.fill(a, table);
+        __builtin_amdgcn_wave_barrier();
+        if (p.rotated)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) cs[i] = table[8u * p.j + i];
+        const uint64_t next = (item.unit + item.stride) >> item.lg_parts;
+        if (a.R) turns.request(a, next < a.tokens ? next : 0u);
+        do {
             float v[2][8], d[2][8];
-            unpack(rx[0], v[0]);
-            unpack(rx[1], v[1]);
-            unpack(rg[0], d[0]);
-            unpack(rg[1], d[1]);
+            unpack_units(rx, v);
+            unpack_units(rg, d);
             request();
+            float ss = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(v[u][i], v[u][i], ss);
+            ss = lane_group_sum(p.active ? ss : 0.0f, lg);
+            const float rho = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, inv_d, a.eps));
             if (hadamard) {
                 head_butterflies(d, p.j, lg);
 #pragma unroll
@@ -471,40 +528,34 @@ __global__ void __launch_bounds__(256) qk_norm_rope_backward_kernel(HeadsArgs a)
                     for (int i = 0; i < 8; ++i) d[u][i] *= sign;
                 if (mixed) relayout<true>(d, p.lane, p.j, lg, a.R / 16u);
             }
-            if (p.rotated) {
-                float2 cs[8];
+            if (p.rotated) rotate_pairs<-1, NEIGHBOURS>(d, cs);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) cs[i] = table[item.token * half + 8u * p.j + i];
-                rotate_pairs<-1, NEIGHBOURS>(d, cs);
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[u][i] *= rho;  // the normed value
+            if (p.active && item.pass * p.groups + p.group < heads) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dw[u][i] = __builtin_fmaf(d[u][i], v[u][i], dw[u][i]);
             }
-            float ss = 0.0f, dot = 0.0f, dn[2][8];
+            float dot = 0.0f;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    ss = __builtin_fmaf(v[u][i], v[u][i], ss);
-                    dn[u][i] = d[u][i] * v[u][i];
                     d[u][i] *= w[u][i];
                     dot = __builtin_fmaf(d[u][i], v[u][i], dot);
                 }
-            ss = lane_group_sum(ss, lg);
-            dot = lane_group_sum(dot, lg);
-            const float rho = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, inv_d, a.eps));
-            const float back = rho * rho * dot * inv_d;
+            const float mean = lane_group_sum(p.active ? dot : 0.0f, lg) * inv_d;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    dw[u][i] = __builtin_fmaf(dn[u][i], rho, dw[u][i]);
-                    d[u][i] = rho * __builtin_fmaf(-back, v[u][i], d[u][i]);
-                }
-            const uint32_t h = item.pass * p.groups + p.group;
-            if (p.active && h < heads) {
-                E* row = y + item.token * side.y_ts + h * side.y_hs;
-                store_unit(row + p.unit[0], d[0]);
-                store_unit(row + p.unit[1], d[1]);
-            }
-        }
+                for (int i = 0; i < 8; ++i) d[u][i] = rho * __builtin_fmaf(-mean, v[u][i], d[u][i]);
+            E* row = y + item.token() * side.y_ts + p.head(item.pass, heads) * side.y_hs;
+            store_unit(row + p.unit[0], d[0]);
+            store_unit(row + p.unit[1], d[1]);
+        } while (!item.next());
     }
 
     // Weight gradients of the workgroup: over the lane groups, then over the wavefronts, always in the
@@ -610,26 +661,25 @@ int make_args(const mi_heads* d, const void* const* tensors, int count, const vo
     return MI_OK;
 }
 
-// Tokens per workgroup and workgroups of each kind.  Up to 8192 items (the wavefronts that the chip holds)
-// there is one for each wavefront; beyond, up to four, which keeps the table and the weights busy.
-void cut_work(HeadsArgs& a, uint64_t max_blocks)
+// Workgroups of each side, and how many wavefronts share a token.  At most `most` workgroups, which is what the
+// chip holds at once, in proportion to the items; every wavefront of a side has the same number of units but for
+// the last.  Where the tokens alone do not give that many wavefronts, their heads are shared out.
+void cut_work(HeadsArgs& a, uint32_t most)
 {
     const uint32_t groups = 64u >> a.lg;
     Side* const sides[2] = {&a.q, &a.k};
-    uint64_t items = 0, total = 0;
-    for (Side* s : sides) items += a.tokens * ((s->heads + groups - 1u) / groups);
-    const uint32_t per_wave = items <= 8192u ? 1u : items >= 4u * 8192u ? 4u : (uint32_t)(items / 8192u);
-    uint64_t wanted[2];
+    uint64_t items[2];
+    for (int i = 0; i < 2; ++i) items[i] = a.tokens * ((sides[i]->heads + groups - 1u) / groups);
     for (int i = 0; i < 2; ++i) {
-        const uint32_t per_token = (sides[i]->heads + groups - 1u) / groups;
-        uint32_t n = per_token ? 4u * per_wave / per_token : 1u;
-        if (a.R && n > kTableEntries / (a.R / 2u)) n = kTableEntries / (a.R / 2u);
-        sides[i]->per_block = n ? n : 1u;
-        wanted[i] = per_token ? (a.tokens + sides[i]->per_block - 1u) / sides[i]->per_block : 0u;
-        total += wanted[i];
+        Side& s = *sides[i];
+        s.lg_parts = s.blocks = 0;
+        if (!items[i]) continue;
+        const uint32_t per_token = (s.heads + groups - 1u) / groups;
+        const uint64_t waves = 4u * (1u + items[i] * (most - 2u) / (items[0] + items[1]));
+        while ((2u << s.lg_parts) <= per_token && a.tokens << s.lg_parts < waves) ++s.lg_parts;
+        const uint64_t units = a.tokens << s.lg_parts, each = (units + waves - 1u) / waves;
+        s.blocks = (uint32_t)(((units + each - 1u) / each + 3u) / 4u);
     }
-    for (int i = 0; i < 2; ++i)  // in proportion where there are too many
-        sides[i]->blocks = (uint32_t)(total <= max_blocks ? wanted[i] : wanted[i] ? 1u + wanted[i] * (max_blocks - 2u) / total : 0u);
 }
 
 template <bool BACKWARD, class E, int LG, bool NEIGHBOURS>
@@ -680,14 +730,14 @@ extern "C" int mi_qk_norm_rope(const void* q, const void* k, const void* q_weigh
     a.q.w = q_weight;
     a.k.w = k_weight;
     if ((q_weight && !aligned16(q_weight)) || (k_weight && !aligned16(k_weight))) return MI_ERR_ALIGN;
-    cut_work(a, 1ull << 30);
+    cut_work(a, kMaxBlocks);
     return launch_heads<false>(a, d->dtype, static_cast<hipStream_t>(stream));
 }
 
 extern "C" uint64_t mi_qk_norm_rope_workspace(uint64_t tokens, uint32_t head_dim)
 {
     using namespace mi;
-    return (tokens < kMaxPartials / 2u ? 2u * tokens : kMaxPartials) * head_dim * sizeof(float);
+    return tokens ? (uint64_t)kMaxPartials * head_dim * sizeof(float) : 0u;
 }
 
 extern "C" int mi_qk_norm_rope_backward(const void* q, const void* k, const void* q_grad, const void* k_grad, const void* q_weight,
