@@ -82,6 +82,10 @@ __device__ __forceinline__ void half_scale(float m, float& up, float& down)
     down = __builtin_bit_cast(float, (e - 14u) << 23);
 }
 
+// The wavefront's number in a scalar register.  Matrix-core instructions ignore the lane mask, so what decides
+// about them has to be a branch that the whole wavefront takes or does not take.
+__device__ __forceinline__ uint32_t this_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 template <class V>
 __device__ __forceinline__ V load16(const void* p)
 {
@@ -100,68 +104,86 @@ struct ContractArgs {
     const void* M;       // [n][rank][K]
     float* P;            // [splits][tokens][16 RT]
     uint64_t tokens;
-    uint32_t n, rank, K, part;  // part: extent of K per workgroup, a multiple of 8 * STEP
+    uint32_t n, rank, K, splits, part;  // part: extent of K per workgroup, a multiple of 8 * STEP
 };
 
 // P^T tile = M (rows: r) . x^T (columns: tokens).  The four wavefronts take turns along the part of K, two
-// steps (a 128-byte line of every row) at a time, and add their sums through LDS.
+// steps (a 128-byte line of every row) at a time with the next two requested, and add their sums through
+// LDS.  Columns behind the tile's tokens repeat its first one and rows behind the rank the first rank: the
+// loads need no masks, and what they give is not stored.
 template <class E, int RT, int SUB>
-__device__ __forceinline__ void contract_tile(const ContractArgs& a, const Tile& tile, f32x4* red)
+__device__ __forceinline__ void contract_tile(const ContractArgs& a, const Tile& tile, uint32_t split, f32x4* red)
 {
     using X = Mx<E>;
     using V = typename X::V;
     constexpr uint32_t kBlock = 2u * X::STEP;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, lo = lane & 15u, g = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), lo = lane & 15u, g = lane >> 4;
     const PlanLayout L(a.tokens, a.n);
-    const uint32_t k0 = blockIdx.y * a.part;
+    const uint32_t k0 = split * a.part;
     const uint32_t k1 = a.K - k0 < a.part ? a.K : k0 + a.part;
 
     const E* xr[SUB];
 #pragma unroll
     for (int i = 0; i < SUB; ++i) {
-        uint32_t at = 16u * i + lo;
-        if (at >= (uint32_t)tile.count) at = 0;  // a column of its own: its sums are not stored
-        const int32_t t = a.plan[L.order + (uint32_t)tile.first + at];
+        const uint32_t at = 16u * i + lo;
+        const int32_t t = a.plan[L.order + (uint32_t)tile.first + (at < (uint32_t)tile.count ? at : 0u)];
         xr[i] = static_cast<const E*>(a.x.p) + (uint64_t)t * a.x.stride + X::VEC * g;
     }
     const E* mr[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        uint32_t r = 16u * i + lo;
-        if (r >= a.rank) r = 0;  // a row of its own: stored as zeros
-        mr[i] = static_cast<const E*>(a.M) + ((uint64_t)tile.adapter * a.rank + r) * a.K + X::VEC * g;
+        const uint32_t r = 16u * i + lo;
+        mr[i] = static_cast<const E*>(a.M) + ((uint64_t)tile.adapter * a.rank + (r < a.rank ? r : 0u)) * a.K + X::VEC * g;
     }
+    struct Block { V x[2][SUB], m[2][RT]; };
     f32x4 acc[SUB][RT] = {};
-    uint32_t k = k0 + wave * kBlock;
-    for (; k + kBlock <= k1; k += 4u * kBlock) {
-        V xf[2][SUB], mf[2][RT];
+    const uint32_t full = (k1 - k0) / kBlock, mine = full > wave ? (full - wave + 3u) / 4u : 0u;
+    auto load = [&](Block& b, uint32_t i) __attribute__((always_inline)) {
+        const uint32_t k = k0 + (wave + 4u * i) * kBlock;
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int i = 0; i < SUB; ++i) xf[h][i] = load16<V>(xr[i] + k + h * X::STEP);
+            for (int j = 0; j < SUB; ++j) b.x[h][j] = load16<V>(xr[j] + k + h * X::STEP);
 #pragma unroll
-            for (int i = 0; i < RT; ++i) mf[h][i] = load16<V>(mr[i] + k + h * X::STEP);
+            for (int j = 0; j < RT; ++j) b.m[h][j] = load16<V>(mr[j] + k + h * X::STEP);
         }
+    };
+    auto multiply = [&](const Block& b) __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
             for (int j = 0; j < RT; ++j)
 #pragma unroll
-                for (int i = 0; i < SUB; ++i) acc[i][j] = X::mma(mf[h][j], xf[h][i], acc[i][j]);
-    }
-    for (uint32_t h = 0; k < k1 && h < 2; ++h, k += X::STEP) {  // the end of K, in the wavefront that it falls to
-        const bool in = k + X::VEC * g < k1;
-        V xf[SUB] = {}, mf[RT] = {};
-        if (in) {
-#pragma unroll
-            for (int i = 0; i < SUB; ++i) xf[i] = load16<V>(xr[i] + k);
-#pragma unroll
-            for (int i = 0; i < RT; ++i) mf[i] = load16<V>(mr[i] + k);
+                for (int i = 0; i < SUB; ++i) acc[i][j] = X::mma(b.m[h][j], b.x[h][i], acc[i][j]);
+    };
+    if (mine) {
+        Block p, q;
+        uint32_t i = 0;
+        load(p, 0);
+        for (; i + 2u < mine; i += 2u) {
+            load(q, i + 1u);
+            multiply(p);
+            load(p, i + 2u);
+            multiply(q);
         }
+        if (i + 1u < mine) load(q, i + 1u);
+        multiply(p);
+        if (i + 1u < mine) multiply(q);
+    }
+    if ((full & 3u) == wave) {  // the rest of K: less than a block, values behind the end are zeros on both sides
+        for (uint32_t k = k0 + full * kBlock; k < k1; k += X::STEP) {
+            V xf[SUB] = {}, mf[RT] = {};
+            if (k + X::VEC * g < k1) {
 #pragma unroll
-        for (int j = 0; j < RT; ++j)
+                for (int i = 0; i < SUB; ++i) xf[i] = load16<V>(xr[i] + k);
 #pragma unroll
-            for (int i = 0; i < SUB; ++i) acc[i][j] = X::mma(mf[j], xf[i], acc[i][j]);
+                for (int i = 0; i < RT; ++i) mf[i] = load16<V>(mr[i] + k);
+            }
+#pragma unroll
+            for (int j = 0; j < RT; ++j)
+#pragma unroll
+                for (int i = 0; i < SUB; ++i) acc[i][j] = X::mma(mf[j], xf[i], acc[i][j]);
+        }
     }
     // wavefronts 2, 3 to 0, 1, then 1 to 0
 #pragma unroll
@@ -182,7 +204,7 @@ __device__ __forceinline__ void contract_tile(const ContractArgs& a, const Tile&
         __syncthreads();
     }
     if (wave) return;
-    float* P = a.P + ((uint64_t)blockIdx.y * a.tokens + (uint32_t)tile.first) * (16u * RT);
+    float* P = a.P + ((uint64_t)split * a.tokens + (uint32_t)tile.first) * (16u * RT);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < SUB; ++i)
@@ -193,23 +215,45 @@ __device__ __forceinline__ void contract_tile(const ContractArgs& a, const Tile&
                     16u * j + 4u * g < a.rank ? acc[i][j] : zero;
 }
 
-template <class E, int RT>
-__global__ void __launch_bounds__(256) contract_rows_kernel(ContractArgs a)
+// The work of a workgroup: a tile, or with FEW 16 of its tokens, and one of `parts` parts of an axis.  Consecutive
+// workgroups take the parts of one tile: they run on different XCDs, so an XCD's L2 holds its part of the
+// adapters for all tiles.  False where the plan has no such tile.
+template <bool FEW>
+__device__ __forceinline__ bool take_tile(const int32_t* plan, const PlanLayout& L, uint32_t parts, Tile& tile, uint32_t& part)
 {
-    __shared__ f32x4 red[2 * 4 * RT * 64];
+    uint32_t t = blockIdx.x / parts, sub = 0;
+    part = blockIdx.x - t * parts;
+    if (FEW) {
+        sub = 16u * (t & 3u);
+        t >>= 2;
+    }
+    tile = reinterpret_cast<const Tile*>(plan)[t];
+    if (t >= (uint32_t)plan[L.counts]) return false;
+    if (FEW) {
+        tile.first += (int32_t)sub;
+        tile.count -= (int32_t)sub;
+        if (tile.count > 16) tile.count = 16;
+    }
+    return tile.count > 0;
+}
+
+template <class E, int RT, bool FEW>
+__global__ void __launch_bounds__(256, FEW || RT == 8 ? 1 : 2) contract_rows_kernel(ContractArgs a)
+{
+    __shared__ f32x4 red[2 * (FEW ? 1 : 4) * RT * 64];
     const PlanLayout L(a.tokens, a.n);
-    if (blockIdx.x >= (uint32_t)a.plan[L.counts]) return;
-    const Tile tile = reinterpret_cast<const Tile*>(a.plan)[blockIdx.x];
-    if ((uint32_t)tile.adapter >= a.n) return;
-    if (tile.count <= 16) contract_tile<E, RT, 1>(a, tile, red);
-    else if (tile.count <= 32) contract_tile<E, RT, 2>(a, tile, red);
-    else contract_tile<E, RT, 4>(a, tile, red);
+    Tile tile;
+    uint32_t split;
+    if (!take_tile<FEW>(a.plan, L, a.splits, tile, split) || (uint32_t)tile.adapter >= a.n) return;
+    if constexpr (FEW) contract_tile<E, RT, 1>(a, tile, split, red);
+    else if (tile.count <= 32) contract_tile<E, RT, 2>(a, tile, split, red);
+    else contract_tile<E, RT, 4>(a, tile, split, red);
 }
 
 // ------------------------------------------------------------------------------------------------
 struct ExpandArgs {
     const int32_t* plan;
-    Rows y;              // added to; NULL: nothing is
+    Rows y;              // added to
     void* out;
     uint64_t out_stride;
     const void* M;       // [n][N][rank]
@@ -217,150 +261,234 @@ struct ExpandArgs {
     const float* P;      // [splits][tokens][16 RT]
     float* shrunk;       // [tokens][rank] or NULL: the sums of P in the tokens' own order
     uint64_t tokens;
-    uint32_t n, rank, N, splits, part;  // part: extent of N per workgroup
+    uint32_t n, rank, N, splits, part, parts;  // part: extent of N per workgroup
 };
 
-// out^T tile = M (rows: n) . v^T (columns: tokens), v = s * sum of P held as fragments.  Row m = 4 g + q of
-// the 16-row operand t stands for n = base + VEC g + 4 t + q, so that a lane's results are VEC consecutive
-// values of its token: 16-byte loads of y and stores of out.
-template <class E, int RT, int SUB>
-__device__ __forceinline__ void expand_tile(const ExpandArgs& a, const Tile& tile)
+// The rank-space vectors of a tile as matrix-core operands in LDS: fragment (sub, f, p) of the 16 tokens of
+// sub, the STEP ranks of f (PAIR: all 16 ranks, hi in lane groups 0, 1 and lo in 2, 3) and piece p.
+template <class E, int RT>
+struct Operand {
+    using X = Mx<E>;
+    static constexpr bool PAIR = X::PIECES == 2 && RT == 1;
+    static constexpr int NF = X::PIECES == 2 ? (RT + 1) / 2 : RT;
+    static constexpr int NP = PAIR ? 1 : (int)X::PIECES;
+    static constexpr uint32_t BYTES = 4u * NF * NP * 1024u;
+    // byte offset of piece p of rank r of token t (0 ... 63)
+    static __device__ __forceinline__ uint32_t at(uint32_t t, uint32_t r, uint32_t p)
+    {
+        const uint32_t f = PAIR ? 0u : r / X::STEP, g = PAIR ? r / 8u + 2u * p : r % X::STEP / X::VEC;
+        return (((t >> 4) * NF + f) * NP + (PAIR ? 0u : p)) * 1024u + (16u * g + (t & 15u)) * 16u + r % X::VEC * (uint32_t)sizeof(E);
+    }
+};
+
+// Sums of P, times the factor, split: four threads per token, 4 RT ranks each.  Tokens behind the tile's
+// repeat its first one.
+template <class E, int RT, bool FEW>
+__device__ __forceinline__ void make_operand(const ExpandArgs& a, const Tile& tile, unsigned char* lds, float* down, bool first_part)
 {
     using X = Mx<E>;
-    using V = typename X::V;
-    constexpr uint32_t VEC = X::VEC, NT = VEC / 4u, ROWS = 16u * NT;
-    constexpr bool PAIR = X::PIECES == 2 && RT == 1;           // hi and lo share one step of the contraction
-    constexpr int NF = X::PIECES == 2 ? (RT + 1) / 2 : RT;     // fragments along r
-    constexpr int NP = PAIR ? 1 : (int)X::PIECES;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, lo = lane & 15u, g = lane >> 4;
+    using O = Operand<E, RT>;
+    typedef E E4 __attribute__((ext_vector_type(4)));
     const PlanLayout L(a.tokens, a.n);
+    const uint32_t t = threadIdx.x >> 2, r0 = (threadIdx.x & 3u) * 4u * RT;
+    if (FEW && t >= 16u) return;
+    const bool live = t < (uint32_t)tile.count;
     const float s = a.scales ? a.scales[tile.adapter] : 1.0f;
-
-    V vf[SUB][NF][NP];
-    float down[SUB];
-    int32_t token[SUB];
+    const float* P = a.P + ((uint64_t)(uint32_t)tile.first + (live ? t : 0u)) * (16u * RT) + r0;
+    f32x4 sum[RT] = {};
+#pragma unroll 4
+    for (uint32_t sp = 0; sp < a.splits; ++sp)
 #pragma unroll
-    for (int i = 0; i < SUB; ++i) {
-        const uint32_t at = 16u * i + lo;
-        const bool live = at < (uint32_t)tile.count;
-        token[i] = live ? a.plan[L.order + (uint32_t)tile.first + at] : -1;
-        float v[NF][VEC];
+        for (int i = 0; i < RT; ++i) sum[i] += load16<f32x4>(P + (uint64_t)sp * a.tokens * (16u * RT) + 4 * i);
+    if (a.shrunk && first_part && live) {
+        float* u = a.shrunk + (uint64_t)(uint32_t)a.plan[L.order + (uint32_t)tile.first + t] * a.rank;
 #pragma unroll
-        for (int f = 0; f < NF; ++f) {
-            const uint32_t r0 = PAIR ? 8u * (g & 1u) : X::STEP * f + VEC * g;
-            float sum[VEC] = {};
-            if (live) {
-                const float* P = a.P + ((uint64_t)(uint32_t)tile.first + at) * (16u * RT) + r0;
-                for (uint32_t sp = 0; sp < a.splits; ++sp, P += a.tokens * (16u * RT))
+        for (int i = 0; i < RT; ++i)
+            if (r0 + 4u * i < a.rank)
 #pragma unroll
-                    for (uint32_t e = 0; e < VEC; e += 4) {
-                        const f32x4 q = load16<f32x4>(P + e);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) sum[e + c] += q[c];
-                    }
-                if (a.shrunk && blockIdx.y == 0 && wave == 0 && r0 < a.rank && !(PAIR && g >= 2u)) {
-                    float* u = a.shrunk + (uint64_t)token[i] * a.rank + r0;
-#pragma unroll
-                    for (uint32_t e = 0; e < VEC; ++e) u[e] = sum[e];
-                }
-            }
-#pragma unroll
-            for (uint32_t e = 0; e < VEC; ++e) v[f][e] = sum[e] * s;
-        }
-        float up = 1.0f;
-        down[i] = 1.0f;
-        if constexpr (X::SCALED) {
-            float m = 0.0f;
-#pragma unroll
-            for (int f = 0; f < NF; ++f)
-#pragma unroll
-                for (uint32_t e = 0; e < VEC; ++e) m = fmaxf(m, finite_magnitude(v[f][e]));
-            m = fmaxf(m, __shfl_xor(m, 16));
-            m = fmaxf(m, __shfl_xor(m, 32));
-            half_scale(m, up, down[i]);
-        }
-#pragma unroll
-        for (int f = 0; f < NF; ++f)
-#pragma unroll
-            for (uint32_t e = 0; e < VEC; ++e) {
-                if constexpr (X::PIECES == 1) {
-                    vf[i][f][0][e] = v[f][e];
-                } else {
-                    E hi, low;
-                    split<E>(v[f][e] * up, hi, low);
-                    if constexpr (PAIR) vf[i][f][0][e] = g < 2u ? hi : low;
-                    else { vf[i][f][0][e] = hi; vf[i][f][1][e] = low; }
-                }
-            }
+                for (int c = 0; c < 4; ++c) u[r0 + 4u * i + c] = sum[i][c];
     }
-
-    const uint32_t n0 = blockIdx.y * a.part;
-    const uint32_t n1 = a.N - n0 < a.part ? a.N : n0 + a.part;
-    const E* M = static_cast<const E*>(a.M) + (uint64_t)tile.adapter * a.N * a.rank;
-    for (uint32_t nb = n0 + wave * ROWS; nb < n1; nb += 4u * ROWS) {
-        V mf[NT][NF] = {};
+    float up = 1.0f;
 #pragma unroll
-        for (uint32_t t = 0; t < NT; ++t) {
-            const uint32_t row = nb + VEC * (lo >> 2) + 4u * t + (lo & 3u);
+    for (int i = 0; i < RT; ++i) sum[i] = sum[i] * s;
+    if constexpr (X::SCALED) {
+        float m = 0.0f, d;
 #pragma unroll
-            for (int f = 0; f < NF; ++f) {
-                const uint32_t r0 = PAIR ? 8u * (g & 1u) : X::STEP * f + VEC * g;
-                if (row < n1 && r0 < a.rank) mf[t][f] = load16<V>(M + (uint64_t)row * a.rank + r0);
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) m = fmaxf(m, finite_magnitude(sum[i][c]));
+        m = fmaxf(m, __shfl_xor(m, 1));
+        m = fmaxf(m, __shfl_xor(m, 2));
+        half_scale(m, up, d);
+        if ((threadIdx.x & 3u) == 0) down[t] = d;
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        if constexpr (X::PIECES == 1) {
+            *reinterpret_cast<f32x4*>(lds + O::at(t, r0 + 4u * i, 0)) = sum[i];
+        } else {
+            E4 hi, low;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                E h, l;
+                split<E>(sum[i][c] * up, h, l);
+                hi[c] = h;
+                low[c] = l;
             }
-        }
-        const uint32_t col = nb + VEC * g;
-#pragma unroll
-        for (int i = 0; i < SUB; ++i) {
-            const bool live = token[i] >= 0 && col < n1;
-            V y = {};
-            if (live && a.y.p) y = load16<V>(static_cast<const E*>(a.y.p) + (uint64_t)token[i] * a.y.stride + col);
-            f32x4 acc[NT] = {};
-#pragma unroll
-            for (int f = 0; f < NF; ++f)
-#pragma unroll
-                for (int p = 0; p < NP; ++p)
-#pragma unroll
-                    for (uint32_t t = 0; t < NT; ++t) acc[t] = X::mma(mf[t][f], vf[i][f][p], acc[t]);
-            if (live) {
-                V o;
-#pragma unroll
-                for (uint32_t e = 0; e < VEC; ++e) o[e] = (E)__builtin_fmaf(acc[e / 4u][e % 4u], down[i], (float)y[e]);
-                *reinterpret_cast<V*>(static_cast<E*>(a.out) + (uint64_t)token[i] * a.out_stride + col) = o;
-            }
+            *reinterpret_cast<E4*>(lds + O::at(t, r0 + 4u * i, 0)) = hi;
+            *reinterpret_cast<E4*>(lds + O::at(t, r0 + 4u * i, 1)) = low;
         }
     }
 }
 
-template <class E, int RT>
-__global__ void __launch_bounds__(256) expand_rows_kernel(ExpandArgs a)
+// out^T tile = M (rows: n) . v^T (columns: tokens).  Row m = 4 g + q of the 16-row operand t stands for
+// n = base + VEC g + 4 t + q, so that a lane's results are VEC consecutive values of its token: 16-byte loads
+// of y and stores of out.  A wavefront takes two such bases (a 128-byte line of every token) at a time
+// with the next two requested.  Tokens behind the tile's are its first token again and columns behind N
+// the last VEC ones: these lanes compute and store what the owner does, from a y that was loaded before
+// the owner stores (out may be y), so that no load or store stands behind a branch.
+template <class E, int RT, int SUB, bool HAS_Y>
+__device__ __forceinline__ void expand_tile(const ExpandArgs& a, const Tile& tile, uint32_t part, const unsigned char* lds, const float* down)
+{
+    using X = Mx<E>;
+    using V = typename X::V;
+    using O = Operand<E, RT>;
+    constexpr uint32_t VEC = X::VEC, NT = VEC / 4u, ROWS = 16u * NT;
+    constexpr uint32_t U = X::PIECES == 1 && RT == 8 ? 1 : 2, BLOCK = U * ROWS;  // fp32 of rank 128: one base, as the registers allow
+    constexpr int NF = O::NF, NP = O::NP;
+    const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), lo = lane & 15u, g = lane >> 4;
+    const PlanLayout L(a.tokens, a.n);
+    const uint32_t n0 = part * a.part;
+    const uint32_t n1 = a.N - n0 < a.part ? a.N : n0 + a.part;
+    const uint32_t blocks = (n1 - n0 + BLOCK - 1u) / BLOCK, mine = blocks > wave ? (blocks - wave + 3u) / 4u : 0u;
+    const bool ragged = a.rank != 16u * RT;
+
+    const E* yr[SUB];
+    E* outr[SUB];
+#pragma unroll
+    for (int i = 0; i < SUB; ++i) {
+        const uint32_t at = 16u * i + lo;
+        const uint64_t t = (uint64_t)(uint32_t)a.plan[L.order + (uint32_t)tile.first + (at < (uint32_t)tile.count ? at : 0u)];
+        yr[i] = static_cast<const E*>(a.y.p) + t * a.y.stride;
+        outr[i] = static_cast<E*>(a.out) + t * a.out_stride;
+    }
+    const E* M = static_cast<const E*>(a.M) + (uint64_t)tile.adapter * a.N * a.rank;
+    uint32_t r0[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        r0[f] = O::PAIR ? 8u * (g & 1u) : X::STEP * f + VEC * g;
+        if (r0[f] >= a.rank) r0[f] = a.rank;  // zeros
+    }
+    struct Block { V m[U][NT][NF], y[U][SUB]; };
+    auto column = [&](uint32_t i, uint32_t u, uint32_t group) {
+        const uint32_t n = n0 + (wave + 4u * i) * BLOCK + u * ROWS + VEC * group;
+        return n < a.N ? n : a.N - VEC;
+    };
+    auto load = [&](Block& b, uint32_t i) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t row = column(i, u, lo >> 2) + (lo & 3u);
+#pragma unroll
+            for (uint32_t t = 0; t < NT; ++t)
+#pragma unroll
+                for (int f = 0; f < NF; ++f)
+                    b.m[u][t][f] = load16<V>(M + (uint64_t)(row + 4u * t) * a.rank + (r0[f] < a.rank ? r0[f] : 0u));
+            if (HAS_Y)
+#pragma unroll
+                for (int j = 0; j < SUB; ++j) b.y[u][j] = load16<V>(yr[j] + column(i, u, g));
+        }
+    };
+    auto finish = [&](Block& b, uint32_t i) __attribute__((always_inline)) {
+        if (ragged)
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+                for (uint32_t t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int f = 0; f < NF; ++f) b.m[u][t][f] = r0[f] < a.rank ? b.m[u][t][f] : V{};
+#pragma unroll
+        for (int j = 0; j < SUB; ++j) {
+            f32x4 acc[U][NT] = {};
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+#pragma unroll
+                for (int p = 0; p < NP; ++p) {
+                    const V v = *reinterpret_cast<const V*>(lds + ((j * NF + f) * NP + p) * 1024u + lane * 16u);
+#pragma unroll
+                    for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+                        for (uint32_t t = 0; t < NT; ++t) acc[u][t] = X::mma(b.m[u][t][f], v, acc[u][t]);
+                }
+            const float d = X::SCALED ? down[16u * j + lo] : 1.0f;
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                V o;
+#pragma unroll
+                for (uint32_t e = 0; e < VEC; ++e) {
+                    float v = acc[u][e / 4u][e % 4u];
+                    if (HAS_Y) v = X::SCALED ? __builtin_fmaf(v, d, (float)b.y[u][j][e]) : v + (float)b.y[u][j][e];
+                    else if (X::SCALED) v *= d;
+                    o[e] = (E)v;
+                }
+                __builtin_nontemporal_store(o, reinterpret_cast<V*>(outr[j] + column(i, u, g)));
+            }
+        }
+    };
+    if (!mine) return;
+    Block p, q;
+    uint32_t i = 0;
+    load(p, 0);
+    for (; i + 2u < mine; i += 2u) {
+        load(q, i + 1u);
+        finish(p, i);
+        load(p, i + 2u);
+        finish(q, i + 1u);
+    }
+    if (i + 1u < mine) {
+        load(q, i + 1u);
+        finish(p, i);
+        finish(q, i + 1u);
+    } else {
+        finish(p, i);
+    }
+}
+
+template <class E, int RT, bool HAS_Y, bool FEW>
+__global__ void __launch_bounds__(256, FEW || RT == 8 ? 1 : 2) expand_rows_kernel(ExpandArgs a)
 {
     using V = typename Mx<E>::V;
     constexpr uint32_t VEC = Mx<E>::VEC;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[Operand<E, RT>::BYTES];
+    __shared__ float down[64];
     const PlanLayout L(a.tokens, a.n);
-    if (blockIdx.x >= (uint32_t)a.plan[L.counts]) return;
-    const Tile tile = reinterpret_cast<const Tile*>(a.plan)[blockIdx.x];
+    Tile tile;
+    uint32_t part;
+    if (!take_tile<FEW>(a.plan, L, a.parts, tile, part)) return;
     if ((uint32_t)tile.adapter < a.n) {
-        if (tile.count <= 16) expand_tile<E, RT, 1>(a, tile);
-        else if (tile.count <= 32) expand_tile<E, RT, 2>(a, tile);
-        else expand_tile<E, RT, 4>(a, tile);
+        make_operand<E, RT, FEW>(a, tile, lds, down, part == 0u);
+        if (a.N == 0u) return;
+        __syncthreads();
+        if constexpr (FEW) expand_tile<E, RT, 1, HAS_Y>(a, tile, part, lds, down);
+        else if (tile.count <= 32) expand_tile<E, RT, 2, HAS_Y>(a, tile, part, lds, down);
+        else expand_tile<E, RT, 4, HAS_Y>(a, tile, part, lds, down);
         return;
     }
     // tokens without an adapter: y as it is, or zeros
-    const uint32_t n0 = blockIdx.y * a.part;
+    const uint32_t n0 = part * a.part;
     const uint32_t n1 = a.N - n0 < a.part ? a.N : n0 + a.part;
-    if (a.y.p != a.out)
+    if (a.N && (!HAS_Y || a.y.p != a.out))
         for (uint32_t i = threadIdx.x >> 6; i < (uint32_t)tile.count; i += 4u) {
-            const uint64_t t = (uint64_t)a.plan[L.order + (uint32_t)tile.first + i];
+            const uint64_t t = (uint64_t)(uint32_t)a.plan[L.order + (uint32_t)tile.first + i];
             for (uint32_t c = n0 + VEC * (threadIdx.x & 63u); c < n1; c += VEC * 64u) {
                 V v = {};
-                if (a.y.p) v = load16<V>(static_cast<const E*>(a.y.p) + t * a.y.stride + c);
+                if (HAS_Y) v = load16<V>(static_cast<const E*>(a.y.p) + t * a.y.stride + c);
                 *reinterpret_cast<V*>(static_cast<E*>(a.out) + t * a.out_stride + c) = v;
             }
         }
-    if (a.shrunk && blockIdx.y == 0)
+    if (a.shrunk && part == 0u)
         for (uint32_t i = threadIdx.x; i < (uint32_t)tile.count * a.rank; i += kThreads) {
             const uint32_t at = i / a.rank;
-            a.shrunk[(uint64_t)a.plan[L.order + (uint32_t)tile.first + at] * a.rank + (i - at * a.rank)] = 0.0f;
+            a.shrunk[(uint64_t)(uint32_t)a.plan[L.order + (uint32_t)tile.first + at] * a.rank + (i - at * a.rank)] = 0.0f;
         }
 }
 
@@ -418,7 +546,7 @@ __global__ void __launch_bounds__(256) weight_pieces_kernel(PiecesArgs a)
     if (blockIdx.x >= (uint32_t)a.plan[L.counts]) return;
     const Tile tile = reinterpret_cast<const Tile*>(a.plan)[blockIdx.x];
     if ((uint32_t)tile.adapter >= a.n) return;
-    const uint32_t which = blockIdx.y, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t which = blockIdx.y, lane = threadIdx.x & 63u, wave = this_wave();
     const float s = a.scales ? a.scales[tile.adapter] : 1.0f;
     const bool live = lane < (uint32_t)tile.count;
     const uint64_t pos = (uint64_t)(uint32_t)tile.first + lane;
@@ -501,7 +629,7 @@ __global__ void __launch_bounds__(256) weight_rows_kernel(WeightArgs a)
     const PlanLayout L(a.tokens, a.n);
     if (blockIdx.y >= (uint32_t)a.plan[L.counts + 1u]) return;
     const Chunk chunk = reinterpret_cast<const Chunk*>(a.plan + L.chunks)[blockIdx.y];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, lo = lane & 15u, g = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), lo = lane & 15u, g = lane >> 4;
     for (uint32_t i = threadIdx.x; i < (uint32_t)chunk.count; i += kThreads)
         order[i] = a.plan[L.order + (uint32_t)chunk.first + i];
     __syncthreads();
@@ -644,29 +772,26 @@ __global__ void __launch_bounds__(256) weight_sum_kernel(WeightSumArgs a)
 // ------------------------------------------------------------------------------------------------
 uint32_t padded_rank(uint32_t rank) { return rank <= 16u ? 16u : rank <= 32u ? 32u : rank <= 64u ? 64u : 128u; }
 
-// How a contraction of length K is cut: enough workgroups to fill the chip (four per compute unit), each
-// with at least two steps for every wavefront.
-void cut_contraction(uint64_t tiles, uint32_t K, uint32_t step, uint32_t& part, uint32_t& splits)
+// How an axis is cut: `most` workgroups or a little fewer, but no part smaller than a unit; where there are eight
+// parts or more, a multiple of eight, one XCD's share each.
+void cut(uint64_t tiles, uint32_t length, uint32_t unit, uint32_t most, uint32_t& part, uint32_t& parts)
 {
-    const uint32_t unit = 8u * step, units = (K + unit - 1u) / unit;
-    uint64_t want = tiles ? 1024u / tiles : 1u;
+    const uint32_t units = (length + unit - 1u) / unit;
+    uint64_t want = tiles && units ? most / tiles : 1u;
     if (want < 1u) want = 1u;
-    if (want > units) want = units;
+    if (want > units) want = units ? units : 1u;
+    if (want > 8u) want = want / 8u * 8u;
     part = (units + (uint32_t)want - 1u) / (uint32_t)want * unit;
-    splits = (K + part - 1u) / part;
+    if (!part) part = unit;
+    parts = length ? (length + part - 1u) / part : 1u;
 }
 
-// How the output's N is cut: about four workgroups per compute unit, each with whole 4-wavefront rounds.
-void cut_output(uint64_t tiles, uint32_t N, uint32_t& part, uint32_t& parts)
-{
-    const uint32_t unit = 128u, units = (N + unit - 1u) / unit;
-    uint64_t want = tiles ? 1024u / tiles : 1u;
-    if (want < 1u) want = 1u;
-    if (want > units) want = units;
-    part = (units + (uint32_t)want - 1u) / (uint32_t)want * unit;
-    parts = (N + part - 1u) / part;
-}
-
+#ifndef MC
+#define MC 512u
+#endif
+#ifndef ME
+#define ME 1024u
+#endif
 template <class F>
 void for_rank(uint32_t rp, F f)
 {
@@ -693,26 +818,32 @@ int check(const mi_lora* d)
     return MI_OK;
 }
 
-// The forward pass's workspace: the partial sums P.
+// How a batch is cut, and the forward pass's workspace: the partial sums P.  With few tokens for each adapter
+// (16 on the average, or 256 in all) workgroups take 16 tokens instead of 64: a fourth of the registers, so
+// that four times as many wavefronts hide the latencies that such a batch consists of.
 struct ForwardPlan {
+    bool few;
     uint32_t rp, part, splits, npart, nparts;
-    uint64_t tiles, bytes;
-    explicit ForwardPlan(const mi_lora* d, uint32_t K, uint32_t N)
+    uint64_t tiles, bytes;  // tiles: that the grids provide for, absent ones among them
+    ForwardPlan(const mi_lora* d, uint32_t K, uint32_t N)
     {
         const PlanLayout L(d->tokens, d->n_adapters);
+        few = d->tokens <= 256u || d->tokens <= 16u * d->n_adapters;
         tiles = L.max_tiles;
         rp = padded_rank(d->rank);
-        cut_contraction(tiles, K, 4u * elements_of(d->dtype), part, splits);
-        cut_output(tiles, N, npart, nparts);
+        const uint32_t step = 4u * elements_of(d->dtype);
+        cut(tiles, K, 8u * step, few ? 1024u : MC, part, splits);  // each wavefront two blocks of two steps at least
+        cut(tiles, N, 8u * step, few ? 1024u : ME, npart, nparts);  // each wavefront a 128-byte line at least
+        if (few) tiles *= 4u;
         bytes = up256((uint64_t)splits * d->tokens * rp * 4u);
     }
 };
 
 struct BackwardPlan {
     ForwardPlan f;  // contraction over N, expansion to K
-    ForwardPlan u;  // contraction over K, when the forward pass's sums are not given
+    ForwardPlan u;  // contraction over K alone, when the forward pass's sums are not given
     uint64_t at, bt, shrunk, pieces[2], down, partials, bytes;
-    explicit BackwardPlan(const mi_lora* d) : f(d, d->N, d->K), u(d, d->K, 8u)
+    explicit BackwardPlan(const mi_lora* d) : f(d, d->N, d->K), u(d, d->K, 0u)
     {
         const PlanLayout L(d->tokens, d->n_adapters);
         const uint64_t e = d->dtype == MI_F32 ? 4u : 2u, pieces_n = d->dtype == MI_F32 ? 1u : 2u;
@@ -731,9 +862,12 @@ struct BackwardPlan {
 template <class E>
 int contract(const mi_lora* d, const int32_t* plan, Rows x, const void* M, uint32_t K, const ForwardPlan& f, float* P, hipStream_t s)
 {
-    ContractArgs a{plan, x, M, P, d->tokens, d->n_adapters, d->rank, K, f.part};
+    ContractArgs a{plan, x, M, P, d->tokens, d->n_adapters, d->rank, K, f.splits, f.part};
     for_rank(f.rp, [&](auto rt) {
-        hipLaunchKernelGGL((contract_rows_kernel<E, decltype(rt)::value>), dim3((uint32_t)f.tiles, f.splits), dim3(kThreads), 0, s, a);
+        constexpr int RT = decltype(rt)::value;
+        const dim3 grid((uint32_t)f.tiles * f.splits);
+        if (f.few) hipLaunchKernelGGL((contract_rows_kernel<E, RT, true>), grid, dim3(kThreads), 0, s, a);
+        else hipLaunchKernelGGL((contract_rows_kernel<E, RT, false>), grid, dim3(kThreads), 0, s, a);
     });
     return launch_status();
 }
@@ -742,9 +876,14 @@ template <class E>
 int expand(const mi_lora* d, const int32_t* plan, Rows y, void* out, uint64_t out_stride, const void* M, uint32_t N, const float* scales,
            const ForwardPlan& f, const float* P, float* shrunk, hipStream_t s)
 {
-    ExpandArgs a{plan, y, out, out_stride, M, scales, P, shrunk, d->tokens, d->n_adapters, d->rank, N, f.splits, f.npart};
+    ExpandArgs a{plan, y, out, out_stride, M, scales, P, shrunk, d->tokens, d->n_adapters, d->rank, N, f.splits, f.npart, f.nparts};
+    const dim3 grid((uint32_t)f.tiles * f.nparts);
     for_rank(f.rp, [&](auto rt) {
-        hipLaunchKernelGGL((expand_rows_kernel<E, decltype(rt)::value>), dim3((uint32_t)f.tiles, f.nparts), dim3(kThreads), 0, s, a);
+        constexpr int RT = decltype(rt)::value;
+        if (y.p && f.few) hipLaunchKernelGGL((expand_rows_kernel<E, RT, true, true>), grid, dim3(kThreads), 0, s, a);
+        else if (y.p) hipLaunchKernelGGL((expand_rows_kernel<E, RT, true, false>), grid, dim3(kThreads), 0, s, a);
+        else if (f.few) hipLaunchKernelGGL((expand_rows_kernel<E, RT, false, true>), grid, dim3(kThreads), 0, s, a);
+        else hipLaunchKernelGGL((expand_rows_kernel<E, RT, false, false>), grid, dim3(kThreads), 0, s, a);
     });
     return launch_status();
 }
@@ -765,12 +904,8 @@ int backward(const mi_lora* d, const void* dy, const void* x, const void* A, con
     if (!shrunk) {  // u again
         if ((st = contract<E>(d, plan, rx, A, d->K, b.u, P, s)) != MI_OK) return st;
         float* u = reinterpret_cast<float*>(ws + b.shrunk);
-        // the sums into the tokens' order: an expansion of no columns
-        ExpandArgs e{plan, {nullptr, 0}, nullptr, 0, A, nullptr, P, u, d->tokens, d->n_adapters, d->rank, 0, b.u.splits, 8u};
-        for_rank(b.u.rp, [&](auto rt) {
-            hipLaunchKernelGGL((expand_rows_kernel<E, decltype(rt)::value>), dim3((uint32_t)b.u.tiles, 1), dim3(kThreads), 0, s, e);
-        });
-        if ((st = launch_status()) != MI_OK) return st;
+        // the sums into the tokens' order: an expansion to no columns
+        if ((st = expand<E>(d, plan, {nullptr, 0}, nullptr, 0, A, 0, nullptr, b.u, P, u, s)) != MI_OK) return st;
         shrunk = u;
     }
     const uint32_t across = (d->rank + 63u) / 64u;
