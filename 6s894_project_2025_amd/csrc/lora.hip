@@ -15,7 +15,7 @@
 //   expand_rows     out = y + s (sum of P) M'[a]^T:  the forward output, and dx
 //   transpose       B^T and A^T of the adapters in use, which give the backward pass the layouts of the
 //                   forward one
-//   weight_pieces   d and s u, transposed and split, for the contraction over tokens
+//   tile_vectors    the sums of P times s, split, as operands of expand_rows and, transposed, of weight_rows
 //   weight_rows     dA and dB of up to 512 tokens;  weight_sum adds these up
 // All sums are in a fixed order.
 #include <type_traits>
@@ -26,6 +26,14 @@ namespace mi {
 namespace adapters {
 namespace {
 
+#ifndef WE
+#define WE 2
+#endif
+#ifdef NTL
+#define LOADY(V, p) __builtin_nontemporal_load(reinterpret_cast<const V*>(p))
+#else
+#define LOADY(V, p) load16<V>(p)
+#endif
 constexpr uint32_t kThreads = 256;
 
 // A matrix-core step on 16-byte fragments: lane l holds row (or column) l % 16 and the VEC values of the
@@ -104,116 +112,8 @@ struct ContractArgs {
     const void* M;       // [n][rank][K]
     float* P;            // [splits][tokens][16 RT]
     uint64_t tokens;
-    uint32_t n, rank, K, splits, part;  // part: extent of K per workgroup, a multiple of 8 * STEP
+    uint32_t n, rank, K, splits;  // workgroup `split` takes every splits-th block of K
 };
-
-// P^T tile = M (rows: r) . x^T (columns: tokens).  The four wavefronts take turns along the part of K, two
-// steps (a 128-byte line of every row) at a time with the next two requested, and add their sums through
-// LDS.  Columns behind the tile's tokens repeat its first one and rows behind the rank the first rank: the
-// loads need no masks, and what they give is not stored.
-template <class E, int RT, int SUB>
-__device__ __forceinline__ void contract_tile(const ContractArgs& a, const Tile& tile, uint32_t split, f32x4* red)
-{
-    using X = Mx<E>;
-    using V = typename X::V;
-    constexpr uint32_t kBlock = 2u * X::STEP;
-    const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), lo = lane & 15u, g = lane >> 4;
-    const PlanLayout L(a.tokens, a.n);
-    const uint32_t k0 = split * a.part;
-    const uint32_t k1 = a.K - k0 < a.part ? a.K : k0 + a.part;
-
-    const E* xr[SUB];
-#pragma unroll
-    for (int i = 0; i < SUB; ++i) {
-        const uint32_t at = 16u * i + lo;
-        const int32_t t = a.plan[L.order + (uint32_t)tile.first + (at < (uint32_t)tile.count ? at : 0u)];
-        xr[i] = static_cast<const E*>(a.x.p) + (uint64_t)t * a.x.stride + X::VEC * g;
-    }
-    const E* mr[RT];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const uint32_t r = 16u * i + lo;
-        mr[i] = static_cast<const E*>(a.M) + ((uint64_t)tile.adapter * a.rank + (r < a.rank ? r : 0u)) * a.K + X::VEC * g;
-    }
-    struct Block { V x[2][SUB], m[2][RT]; };
-    f32x4 acc[SUB][RT] = {};
-    const uint32_t full = (k1 - k0) / kBlock, mine = full > wave ? (full - wave + 3u) / 4u : 0u;
-    auto load = [&](Block& b, uint32_t i) __attribute__((always_inline)) {
-        const uint32_t k = k0 + (wave + 4u * i) * kBlock;
-#pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int j = 0; j < SUB; ++j) b.x[h][j] = load16<V>(xr[j] + k + h * X::STEP);
-#pragma unroll
-            for (int j = 0; j < RT; ++j) b.m[h][j] = load16<V>(mr[j] + k + h * X::STEP);
-        }
-    };
-    auto multiply = [&](const Block& b) __attribute__((always_inline)) {
-#pragma unroll
-        for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < RT; ++j)
-#pragma unroll
-                for (int i = 0; i < SUB; ++i) acc[i][j] = X::mma(b.m[h][j], b.x[h][i], acc[i][j]);
-    };
-    if (mine) {
-        Block p, q;
-        uint32_t i = 0;
-        load(p, 0);
-        for (; i + 2u < mine; i += 2u) {
-            load(q, i + 1u);
-            multiply(p);
-            load(p, i + 2u);
-            multiply(q);
-        }
-        if (i + 1u < mine) load(q, i + 1u);
-        multiply(p);
-        if (i + 1u < mine) multiply(q);
-    }
-    if ((full & 3u) == wave) {  // the rest of K: less than a block, values behind the end are zeros on both sides
-        for (uint32_t k = k0 + full * kBlock; k < k1; k += X::STEP) {
-            V xf[SUB] = {}, mf[RT] = {};
-            if (k + X::VEC * g < k1) {
-#pragma unroll
-                for (int i = 0; i < SUB; ++i) xf[i] = load16<V>(xr[i] + k);
-#pragma unroll
-                for (int i = 0; i < RT; ++i) mf[i] = load16<V>(mr[i] + k);
-            }
-#pragma unroll
-            for (int j = 0; j < RT; ++j)
-#pragma unroll
-                for (int i = 0; i < SUB; ++i) acc[i][j] = X::mma(mf[j], xf[i], acc[i][j]);
-        }
-    }
-    // wavefronts 2, 3 to 0, 1, then 1 to 0
-#pragma unroll
-    for (uint32_t half = 2; half; half >>= 1) {
-        if (wave >= half && wave < 2u * half) {
-#pragma unroll
-            for (int i = 0; i < SUB; ++i)
-#pragma unroll
-                for (int j = 0; j < RT; ++j) red[(((wave - half) * SUB + i) * RT + j) * 64u + lane] = acc[i][j];
-        }
-        __syncthreads();
-        if (wave < half) {
-#pragma unroll
-            for (int i = 0; i < SUB; ++i)
-#pragma unroll
-                for (int j = 0; j < RT; ++j) acc[i][j] += red[((wave * SUB + i) * RT + j) * 64u + lane];
-        }
-        __syncthreads();
-    }
-    if (wave) return;
-    float* P = a.P + ((uint64_t)split * a.tokens + (uint32_t)tile.first) * (16u * RT);
-    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < SUB; ++i)
-        if (16u * i + lo < (uint32_t)tile.count)
-#pragma unroll
-            for (int j = 0; j < RT; ++j)
-                *reinterpret_cast<f32x4*>(P + (16u * i + lo) * (16u * RT) + 16u * j + 4u * g) =
-                    16u * j + 4u * g < a.rank ? acc[i][j] : zero;
-}
 
 // The work of a workgroup: a tile, or with FEW 16 of its tokens, and one of `parts` parts of an axis.  Consecutive
 // workgroups take the parts of one tile: they run on different XCDs, so an XCD's L2 holds its part of the
@@ -237,17 +137,327 @@ __device__ __forceinline__ bool take_tile(const int32_t* plan, const PlanLayout&
     return tile.count > 0;
 }
 
+// P^T tile = M (rows: r) . x^T (columns: tokens), in blocks of 256 bytes of every row, which is how x and M are
+// read (16 lanes a row) on their way into LDS; there the 16-byte pieces of row i are permuted by i, so that 16
+// rows' pieces of one column come from 16 different banks groups.  The workgroup's wavefronts take 16 tokens
+// each and share the block of M, which has two buffers; with FEW they take every fourth block for the same 16
+// tokens, each with its own M, and add up at the end.  The next block is requested before the present one is
+// computed.  Columns behind the tile's tokens repeat the first of the 16 and rows behind the rank the first
+// rank: the loads need no masks, and what they give is not stored.  LIVE: the wavefront has tokens.
 template <class E, int RT, bool FEW>
-__global__ void __launch_bounds__(256, FEW || RT == 8 ? 1 : 2) contract_rows_kernel(ContractArgs a)
+struct Contraction {
+    static constexpr uint32_t COLS = 256u / sizeof(E);            // k of a block
+    static constexpr uint32_t ROWS_X = 16u * 256u;                // bytes of a wavefront's x
+    static constexpr uint32_t ROWS_M = 16u * RT * 256u;           // bytes of M of a block
+    static constexpr uint32_t LDS = 4u * ROWS_X + (FEW ? 4u : 2u) * ROWS_M;
+    static __device__ __forceinline__ uint32_t at(uint32_t row, uint32_t piece) { return row * 256u + ((piece ^ row) & 15u) * 16u; }
+};
+
+template <class E, int RT, bool FEW, bool LIVE>
+__device__ __forceinline__ void contract_blocks(const ContractArgs& a, const Tile& tile, uint32_t split, unsigned char* lds)
 {
-    __shared__ f32x4 red[2 * (FEW ? 1 : 4) * RT * 64];
+    using X = Mx<E>;
+    using V = typename X::V;
+    using C = Contraction<E, RT, FEW>;
+    constexpr uint32_t VEC = X::VEC, MROWS = FEW ? 4u : 16u, MLOADS = 16u * RT / MROWS;  // rows of M per round of loads, rounds
+    const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), lo = lane & 15u, g = lane >> 4;
+    const PlanLayout L(a.tokens, a.n);
+    // every step-th block of K from the first
+    const uint32_t all = (a.K + C::COLS - 1u) / C::COLS, first = FEW ? split + a.splits * wave : split, step = FEW ? 4u * a.splits : a.splits;
+    const uint32_t blocks = all > first ? (all - first + step - 1u) / step : 0u;
+    const uint32_t sub = FEW ? 0u : 16u * wave;
+    unsigned char* const xl = lds + wave * C::ROWS_X;
+    unsigned char* const ml = lds + 4u * C::ROWS_X + (FEW ? wave * C::ROWS_M : 0u);
+
+    const E* xr[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t at = sub + 4u * j + g;
+        const int32_t t = LIVE ? a.plan[L.order + (uint32_t)tile.first + (at < (uint32_t)tile.count ? at : sub)] : 0;
+        xr[j] = static_cast<const E*>(a.x.p) + (uint64_t)(uint32_t)t * a.x.stride;
+    }
+    const uint32_t mrow = FEW ? g : threadIdx.x >> 4;
+    const E* M = static_cast<const E*>(a.M) + (uint64_t)tile.adapter * a.rank * a.K;
+
+    u32x4 xs[4], ms[MLOADS];
+    auto column = [&](uint32_t i) { return (first + step * i) * C::COLS + VEC * lo; };
+    auto request = [&](uint32_t i) __attribute__((always_inline)) {
+        const uint32_t k = column(i) < a.K ? column(i) : 0u;
+        if (LIVE)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) xs[j] = load16<u32x4>(xr[j] + k);
+#pragma unroll
+        for (uint32_t j = 0; j < MLOADS; ++j) {
+            const uint32_t r = mrow + MROWS * j;
+            ms[j] = load16<u32x4>(M + (uint64_t)(r < a.rank ? r : 0u) * a.K + k);
+        }
+    };
+    auto stage = [&](uint32_t i, unsigned char* to) __attribute__((always_inline)) {
+        const u32x4 zero = {0u, 0u, 0u, 0u};
+        const bool in = column(i) < a.K;
+        if (LIVE)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(xl + C::at(4u * j + g, lo)) = in ? xs[j] : zero;
+#pragma unroll
+        for (uint32_t j = 0; j < MLOADS; ++j) *reinterpret_cast<u32x4*>(to + C::at(mrow + MROWS * j, lo)) = in ? ms[j] : zero;
+    };
+    f32x4 acc[RT] = {};
+    auto compute = [&](const unsigned char* from) __attribute__((always_inline)) {
+        if (!LIVE) return;
+#pragma unroll
+        for (uint32_t h = 0; h < 4; ++h) {
+            const V x = *reinterpret_cast<const V*>(xl + C::at(lo, 4u * h + g));
+#pragma unroll
+            for (uint32_t j = 0; j < RT; ++j) acc[j] = X::mma(*reinterpret_cast<const V*>(from + C::at(16u * j + lo, 4u * h + g)), x, acc[j]);
+        }
+    };
+    auto meet = [&]() __attribute__((always_inline)) {
+        if (FEW) __builtin_amdgcn_wave_barrier();
+        else __syncthreads();
+    };
+    if (blocks) {
+        request(0);
+        stage(0, ml);
+        meet();
+        uint32_t at = 0;
+        for (uint32_t i = 0; i + 1u < blocks; ++i) {
+            request(i + 1u);
+            compute(ml + at);
+            if (!FEW) at ^= C::ROWS_M;
+            __builtin_amdgcn_wave_barrier();  // x is the wavefront's own
+            stage(i + 1u, ml + at);
+            meet();
+        }
+        compute(ml + at);
+    }
+    if constexpr (FEW) {  // wavefronts 2, 3 to 0, 1, then 1 to 0
+        f32x4* const red = reinterpret_cast<f32x4*>(lds);
+        __syncthreads();
+#pragma unroll
+        for (uint32_t half = 2; half; half >>= 1) {
+            if (wave >= half && wave < 2u * half) {
+#pragma unroll
+                for (int j = 0; j < RT; ++j) red[((wave - half) * RT + j) * 64u + lane] = acc[j];
+            }
+            __syncthreads();
+            if (wave < half) {
+#pragma unroll
+                for (int j = 0; j < RT; ++j) acc[j] += red[(wave * RT + j) * 64u + lane];
+            }
+            __syncthreads();
+        }
+        if (wave) return;
+    }
+    if (!LIVE) return;
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    if (sub + lo >= (uint32_t)tile.count) return;
+    float* P = a.P + ((uint64_t)split * a.tokens + (uint32_t)tile.first + sub + lo) * (16u * RT);
+#pragma unroll
+    for (int j = 0; j < RT; ++j) *reinterpret_cast<f32x4*>(P + 16u * j + 4u * g) = 16u * j + 4u * g < a.rank ? acc[j] : zero;
+}
+
+template <class E, int RT, bool FEW>
+__global__ void __launch_bounds__(256, RT == 8 ? 1 : 2) contract_rows_kernel(ContractArgs a)
+{
+    __shared__ __attribute__((aligned(16))) unsigned char lds[Contraction<E, RT, FEW>::LDS];
     const PlanLayout L(a.tokens, a.n);
     Tile tile;
     uint32_t split;
     if (!take_tile<FEW>(a.plan, L, a.splits, tile, split) || (uint32_t)tile.adapter >= a.n) return;
-    if constexpr (FEW) contract_tile<E, RT, 1>(a, tile, split, red);
-    else if (tile.count <= 32) contract_tile<E, RT, 2>(a, tile, split, red);
-    else contract_tile<E, RT, 4>(a, tile, split, red);
+    // every wavefront meets the same barriers on either way
+    if (FEW || 16u * this_wave() < (uint32_t)tile.count) contract_blocks<E, RT, FEW, true>(a, tile, split, lds);
+    else contract_blocks<E, RT, FEW, false>(a, tile, split, lds);
+}
+
+// ------------------------------------------------------------------------------------------------
+// The expansion's matrix-core operands.  out tile = v (rows: 16 tokens) . M^T (columns: n), and column c of the
+// operand t stands for n = base + VEC c + t: a lane's results over t are then VEC consecutive values of a
+// token, and 16 lanes have 256 contiguous bytes of it, which is how y is read and out written.  (With 64
+// contiguous bytes of 16 tokens, the other way round, the address units bound the kernel.)
+template <class E, int RT>
+struct Operand {
+    using X = Mx<E>;
+    static constexpr bool PAIR = X::PIECES == 2 && RT == 1;  // one step: hi in lane groups 0, 1 and lo in 2, 3
+    static constexpr int NF = X::PIECES == 2 ? (RT + 1) / 2 : RT;
+    static constexpr int NP = PAIR ? 1 : (int)X::PIECES;
+    static constexpr uint32_t COLS = 16u * X::VEC;           // n of a block
+    static constexpr uint32_t VECTORS = 4u * NF * NP * 1024u;  // bytes: v of 64 tokens
+    static constexpr uint32_t BLOCK = 16u * RT * 256u;         // bytes: M of a block
+    // byte offset of piece p of rank r of token t (0 ... 63)
+    static __device__ __forceinline__ uint32_t vector_at(uint32_t t, uint32_t r, uint32_t p)
+    {
+        const uint32_t f = PAIR ? 0u : r / X::STEP, g = PAIR ? r / 8u + 2u * p : r % X::STEP / X::VEC;
+        return (((t >> 4) * NF + f) * NP + (PAIR ? 0u : p)) * 1024u + (16u * g + (t & 15u)) * 16u + r % X::VEC * (uint32_t)sizeof(E);
+    }
+    // byte offset of the 16 bytes that lane (c, g) reads for operand t and fragment f.  Rows n and n + 1 of M
+    // come in together and go to operands t and t + 1; the exclusive or spreads them over the banks.
+    static __device__ __forceinline__ uint32_t row_at(uint32_t t, uint32_t f, uint32_t c, uint32_t g)
+    {
+        return (t * NF + f) * (PAIR ? 512u : 1024u) + (16u * g + (c ^ (t | (f & 1u) << 3))) * 16u;
+    }
+};
+
+// The sums of P of four threads per token, 4 RT ranks each (token threadIdx.x / 4).
+template <int RT>
+__device__ __forceinline__ void sum_parts(const float* P, uint64_t tokens, uint32_t splits, uint64_t position, f32x4 (&sum)[RT])
+{
+    P += position * (16u * RT) + (threadIdx.x & 3u) * 4u * RT;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (uint32_t sp = 0; sp < splits; ++sp)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) sum[i] += load16<f32x4>(P + (uint64_t)sp * tokens * (16u * RT) + 4 * i);
+}
+
+template <int RT>
+__device__ __forceinline__ void store_shrunk(float* u, uint32_t rank, const f32x4 (&sum)[RT])
+{
+    const uint32_t r0 = (threadIdx.x & 3u) * 4u * RT;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+        if (r0 + 4u * i < rank)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) u[r0 + 4u * i + c] = sum[i][c];
+}
+
+// A token's vector as the expansion's operand; returns the inverse of its scaling.
+template <class E, int RT>
+__device__ __forceinline__ float store_vector(const f32x4 (&v)[RT], uint32_t t, unsigned char* to)
+{
+    using X = Mx<E>;
+    using O = Operand<E, RT>;
+    typedef E E4 __attribute__((ext_vector_type(4)));
+    const uint32_t r0 = (threadIdx.x & 3u) * 4u * RT;
+    float up = 1.0f, down = 1.0f;
+    if constexpr (X::SCALED) {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) m = fmaxf(m, finite_magnitude(v[i][c]));
+        m = fmaxf(m, __shfl_xor(m, 1));
+        m = fmaxf(m, __shfl_xor(m, 2));
+        half_scale(m, up, down);
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        if constexpr (X::PIECES == 1) {
+            *reinterpret_cast<f32x4*>(to + O::vector_at(t, r0 + 4u * i, 0)) = v[i];
+        } else {
+            E4 hi, low;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                E h, l;
+                split<E>(v[i][c] * up, h, l);
+                hi[c] = h;
+                low[c] = l;
+            }
+            *reinterpret_cast<E4*>(to + O::vector_at(t, r0 + 4u * i, 0)) = hi;
+            *reinterpret_cast<E4*>(to + O::vector_at(t, r0 + 4u * i, 1)) = low;
+        }
+    }
+    return down;
+}
+
+// The source of a tile's token t: tokens behind the tile's repeat the first of their 16, if there is one.
+__device__ __forceinline__ uint32_t source_token(uint32_t t, uint32_t count)
+{
+    return t < count ? t : (t & ~15u) < count ? t & ~15u : 0u;
+}
+
+// ------------------------------------------------------------------------------------------------
+struct VectorArgs {
+    const int32_t* plan;
+    const float* P;        // [splits][tokens][16 RT]
+    const float* scales;   // [n] or NULL
+    float* shrunk;         // NULL, or [tokens][rank]: receives the sums of P; with `given`, holds them
+    unsigned char* vectors;  // NULL, or [tiles][Operand::VECTORS]
+    float* down;             // [tiles][64]
+    void* pieces;            // NULL, or [tiles][16 RT][PIECES][64]: transposed, for the contraction over tokens
+    float* tile_down;        // [tiles]
+    uint64_t tokens;
+    uint32_t n, rank, splits;
+    bool given;
+};
+
+// Where a tile is used by many workgroups: its vectors once, from the sums of P (or from the given ones) times
+// the factor.
+template <class E, int RT>
+__global__ void __launch_bounds__(256) tile_vectors_kernel(VectorArgs a)
+{
+    using X = Mx<E>;
+    using O = Operand<E, RT>;
+    constexpr uint32_t RP = 16u * RT;
+    __shared__ float top[4];
+    __shared__ E turned[RP * X::PIECES * 64u];
+    const PlanLayout L(a.tokens, a.n);
+    const Tile tile = reinterpret_cast<const Tile*>(a.plan)[blockIdx.x];
+    if (blockIdx.x >= (uint32_t)a.plan[L.counts]) return;
+    const uint32_t t = threadIdx.x >> 2, r0 = (threadIdx.x & 3u) * 4u * RT, count = (uint32_t)tile.count;
+    const bool live = t < count;
+    const uint64_t position = (uint64_t)(uint32_t)tile.first + source_token(t, count);
+    const uint64_t token = (uint64_t)(uint32_t)a.plan[L.order + position];
+    if ((uint32_t)tile.adapter >= a.n) {
+        if (a.shrunk && !a.given && live) {
+            f32x4 zero[RT] = {};
+            store_shrunk<RT>(a.shrunk + token * a.rank, a.rank, zero);
+        }
+        return;
+    }
+    const float s = a.scales ? a.scales[tile.adapter] : 1.0f;
+    f32x4 sum[RT] = {};
+    if (a.given) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+            if (r0 + 4u * i < a.rank)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sum[i][c] = a.shrunk[token * a.rank + r0 + 4u * i + c];
+    } else {
+        sum_parts<RT>(a.P, a.tokens, a.splits, position, sum);
+        if (a.shrunk && live) store_shrunk<RT>(a.shrunk + token * a.rank, a.rank, sum);
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) sum[i] = sum[i] * s;
+    if (a.vectors) {
+        const float d = store_vector<E, RT>(sum, t, a.vectors + (uint64_t)blockIdx.x * O::VECTORS);
+        if (X::SCALED && (threadIdx.x & 3u) == 0) a.down[(uint64_t)blockIdx.x * 64u + t] = d;
+    }
+    if (!a.pieces) return;
+    float up = 1.0f;
+    if constexpr (X::SCALED) {
+        float m = 0.0f, d;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) m = fmaxf(m, finite_magnitude(sum[i][c]));
+        for (int w = 1; w < 64; w <<= 1) m = fmaxf(m, __shfl_xor(m, w));
+        if ((threadIdx.x & 63u) == 0) top[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        half_scale(m, up, d);
+        if (threadIdx.x == 0) a.tile_down[blockIdx.x] = d;
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float v = live ? sum[i][c] * up : 0.0f;  // zeros behind the tile's tokens
+            E* to = turned + (r0 + 4u * i + c) * X::PIECES * 64u + t;
+            if constexpr (X::PIECES == 1) {
+                to[0] = v;
+            } else {
+                E hi, low;
+                split<E>(v, hi, low);
+                to[0] = hi;
+                to[64] = low;
+            }
+        }
+    __syncthreads();
+    constexpr uint32_t BYTES = RP * X::PIECES * 64u * sizeof(E);
+    for (uint32_t i = 16u * threadIdx.x; i < BYTES; i += 16u * kThreads)
+        *reinterpret_cast<u32x4*>(static_cast<unsigned char*>(a.pieces) + (uint64_t)blockIdx.x * BYTES + i) =
+            *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(turned) + i);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -257,235 +467,199 @@ struct ExpandArgs {
     void* out;
     uint64_t out_stride;
     const void* M;       // [n][N][rank]
-    const float* scales; // [n] or NULL
-    const float* P;      // [splits][tokens][16 RT]
-    float* shrunk;       // [tokens][rank] or NULL: the sums of P in the tokens' own order
+    const unsigned char* vectors;  // [tiles][Operand::VECTORS], and their
+    const float* down;             // [tiles][64]; not with FEW, which makes them from
+    const float* scales;           // [n] or NULL
+    const float* P;                // [splits][tokens][16 RT], and gives
+    float* shrunk;                 // [tokens][rank] or NULL
     uint64_t tokens;
-    uint32_t n, rank, N, splits, part, parts;  // part: extent of N per workgroup
+    uint32_t n, rank, N, splits, parts;  // workgroup `part` takes every parts-th block of N
 };
 
-// The rank-space vectors of a tile as matrix-core operands in LDS: fragment (sub, f, p) of the 16 tokens of
-// sub, the STEP ranks of f (PAIR: all 16 ranks, hi in lane groups 0, 1 and lo in 2, 3) and piece p.
-template <class E, int RT>
-struct Operand {
-    using X = Mx<E>;
-    static constexpr bool PAIR = X::PIECES == 2 && RT == 1;
-    static constexpr int NF = X::PIECES == 2 ? (RT + 1) / 2 : RT;
-    static constexpr int NP = PAIR ? 1 : (int)X::PIECES;
-    static constexpr uint32_t BYTES = 4u * NF * NP * 1024u;
-    // byte offset of piece p of rank r of token t (0 ... 63)
-    static __device__ __forceinline__ uint32_t at(uint32_t t, uint32_t r, uint32_t p)
-    {
-        const uint32_t f = PAIR ? 0u : r / X::STEP, g = PAIR ? r / 8u + 2u * p : r % X::STEP / X::VEC;
-        return (((t >> 4) * NF + f) * NP + (PAIR ? 0u : p)) * 1024u + (16u * g + (t & 15u)) * 16u + r % X::VEC * (uint32_t)sizeof(E);
-    }
-};
-
-// Sums of P, times the factor, split: four threads per token, 4 RT ranks each.  Tokens behind the tile's
-// repeat its first one.
-template <class E, int RT, bool FEW>
-__device__ __forceinline__ void make_operand(const ExpandArgs& a, const Tile& tile, unsigned char* lds, float* down, bool first_part)
-{
-    using X = Mx<E>;
-    using O = Operand<E, RT>;
-    typedef E E4 __attribute__((ext_vector_type(4)));
-    const PlanLayout L(a.tokens, a.n);
-    const uint32_t t = threadIdx.x >> 2, r0 = (threadIdx.x & 3u) * 4u * RT;
-    if (FEW && t >= 16u) return;
-    const bool live = t < (uint32_t)tile.count;
-    const float s = a.scales ? a.scales[tile.adapter] : 1.0f;
-    const float* P = a.P + ((uint64_t)(uint32_t)tile.first + (live ? t : 0u)) * (16u * RT) + r0;
-    f32x4 sum[RT] = {};
-#pragma unroll 4
-    for (uint32_t sp = 0; sp < a.splits; ++sp)
-#pragma unroll
-        for (int i = 0; i < RT; ++i) sum[i] += load16<f32x4>(P + (uint64_t)sp * a.tokens * (16u * RT) + 4 * i);
-    if (a.shrunk && first_part && live) {
-        float* u = a.shrunk + (uint64_t)(uint32_t)a.plan[L.order + (uint32_t)tile.first + t] * a.rank;
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-            if (r0 + 4u * i < a.rank)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) u[r0 + 4u * i + c] = sum[i][c];
-    }
-    float up = 1.0f;
-#pragma unroll
-    for (int i = 0; i < RT; ++i) sum[i] = sum[i] * s;
-    if constexpr (X::SCALED) {
-        float m = 0.0f, d;
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) m = fmaxf(m, finite_magnitude(sum[i][c]));
-        m = fmaxf(m, __shfl_xor(m, 1));
-        m = fmaxf(m, __shfl_xor(m, 2));
-        half_scale(m, up, d);
-        if ((threadIdx.x & 3u) == 0) down[t] = d;
-    }
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        if constexpr (X::PIECES == 1) {
-            *reinterpret_cast<f32x4*>(lds + O::at(t, r0 + 4u * i, 0)) = sum[i];
-        } else {
-            E4 hi, low;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                E h, l;
-                split<E>(sum[i][c] * up, h, l);
-                hi[c] = h;
-                low[c] = l;
-            }
-            *reinterpret_cast<E4*>(lds + O::at(t, r0 + 4u * i, 0)) = hi;
-            *reinterpret_cast<E4*>(lds + O::at(t, r0 + 4u * i, 1)) = low;
-        }
-    }
-}
-
-// out^T tile = M (rows: n) . v^T (columns: tokens).  Row m = 4 g + q of the 16-row operand t stands for
-// n = base + VEC g + 4 t + q, so that a lane's results are VEC consecutive values of its token: 16-byte loads
-// of y and stores of out.  A wavefront takes two such bases (a 128-byte line of every token) at a time
-// with the next two requested.  Tokens behind the tile's are its first token again and columns behind N
-// the last VEC ones: these lanes compute and store what the owner does, from a y that was loaded before
-// the owner stores (out may be y), so that no load or store stands behind a branch.
-template <class E, int RT, int SUB, bool HAS_Y>
-__device__ __forceinline__ void expand_tile(const ExpandArgs& a, const Tile& tile, uint32_t part, const unsigned char* lds, const float* down)
+// A wavefront's blocks of the part, COLS columns each.  The workgroup's wavefronts take 16 tokens each and share
+// the block of M, which goes through one of two LDS buffers; with FEW each has its own blocks for the same 16
+// tokens, and a buffer of its own.  The next block of M and y is requested before the present one is
+// computed.  LIVE: the wavefront has tokens.  Tokens behind the tile's are the first of the 16 again and
+// columns behind N the last VEC: these lanes compute and store what the owner does, from a y that was loaded
+// before the owner stores (out may be y), so that no load or store stands behind a branch.
+template <class E, int RT, bool HAS_Y, bool FEW, bool LIVE>
+__device__ __forceinline__ void expand_blocks(const ExpandArgs& a, const Tile& tile, uint32_t part, unsigned char* lds,
+                                              const unsigned char* vectors, const float* down)
 {
     using X = Mx<E>;
     using V = typename X::V;
     using O = Operand<E, RT>;
-    constexpr uint32_t VEC = X::VEC, NT = VEC / 4u, ROWS = 16u * NT;
-    constexpr uint32_t U = X::PIECES == 1 && RT == 8 ? 1 : 2, BLOCK = U * ROWS;  // fp32 of rank 128: one base, as the registers allow
+    constexpr uint32_t VEC = X::VEC, COLS = O::COLS;
     constexpr int NF = O::NF, NP = O::NP;
-    const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), lo = lane & 15u, g = lane >> 4;
+    constexpr uint32_t STAGERS = FEW ? 64u : 256u, CHUNKS = 16u * RT * 16u / STAGERS;  // 16-byte pieces of M per thread
+    constexpr uint32_t PER_ROW = 16u * RT / VEC;
+    const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), c = lane & 15u, g = lane >> 4;
     const PlanLayout L(a.tokens, a.n);
-    const uint32_t n0 = part * a.part;
-    const uint32_t n1 = a.N - n0 < a.part ? a.N : n0 + a.part;
-    const uint32_t blocks = (n1 - n0 + BLOCK - 1u) / BLOCK, mine = blocks > wave ? (blocks - wave + 3u) / 4u : 0u;
-    const bool ragged = a.rank != 16u * RT;
+    // every step-th block of N from the first
+    const uint32_t all = (a.N + COLS - 1u) / COLS, first = FEW ? part + a.parts * wave : part, step = FEW ? 4u * a.parts : a.parts;
+    const uint32_t blocks = all > first ? (all - first + step - 1u) / step : 0u;
 
-    const E* yr[SUB];
-    E* outr[SUB];
+    // v of the wavefront's tokens, and where their rows are
+    V vf[NF][NP];
+    const E* yr[4];
+    E* outr[4];
+    float d[4];
+    if (LIVE) {
+        const uint32_t sub = FEW ? 0u : wave;
 #pragma unroll
-    for (int i = 0; i < SUB; ++i) {
-        const uint32_t at = 16u * i + lo;
-        const uint64_t t = (uint64_t)(uint32_t)a.plan[L.order + (uint32_t)tile.first + (at < (uint32_t)tile.count ? at : 0u)];
-        yr[i] = static_cast<const E*>(a.y.p) + t * a.y.stride;
-        outr[i] = static_cast<E*>(a.out) + t * a.out_stride;
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int p = 0; p < NP; ++p) vf[f][p] = *reinterpret_cast<const V*>(vectors + ((sub * NF + f) * NP + p) * 1024u + lane * 16u);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint32_t at = 16u * sub + 4u * g + q;
+            if (at >= (uint32_t)tile.count) at = 16u * sub;
+            const uint64_t t = (uint64_t)(uint32_t)a.plan[L.order + (uint32_t)tile.first + at];
+            yr[q] = static_cast<const E*>(a.y.p) + t * a.y.stride;
+            outr[q] = static_cast<E*>(a.out) + t * a.out_stride;
+            d[q] = X::SCALED ? down[at] : 1.0f;
+        }
     }
+    if (FEW) __syncthreads();  // the buffers of M take the place of the vectors
+    if (FEW && !blocks) return;
+    unsigned char* const buffer = FEW ? lds + wave * O::BLOCK : lds;
+
     const E* M = static_cast<const E*>(a.M) + (uint64_t)tile.adapter * a.N * a.rank;
-    uint32_t r0[NF];
+    auto first_column = [&](uint32_t i) { return (first + step * i) * COLS; };
+    u32x4 staged[CHUNKS];
+    auto request_rows = [&](uint32_t i) __attribute__((always_inline)) {
+        const uint32_t base = first_column(i);
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
-        r0[f] = O::PAIR ? 8u * (g & 1u) : X::STEP * f + VEC * g;
-        if (r0[f] >= a.rank) r0[f] = a.rank;  // zeros
-    }
-    struct Block { V m[U][NT][NF], y[U][SUB]; };
-    auto column = [&](uint32_t i, uint32_t u, uint32_t group) {
-        const uint32_t n = n0 + (wave + 4u * i) * BLOCK + u * ROWS + VEC * group;
+        for (uint32_t k = 0; k < CHUNKS; ++k) {
+            const uint32_t id = (FEW ? lane : threadIdx.x) + k * STAGERS, row = id / PER_ROW, r = id % PER_ROW * VEC;
+            const uint32_t n = base + row < a.N ? base + row : a.N - 1u;  // rows behind N are not read back
+            staged[k] = load16<u32x4>(M + (uint64_t)n * a.rank + (r < a.rank ? r : 0u));
+        }
+    };
+    auto stage_rows = [&](unsigned char* to) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t k = 0; k < CHUNKS; ++k) {
+            const uint32_t id = (FEW ? lane : threadIdx.x) + k * STAGERS, row = id / PER_ROW, r = id % PER_ROW * VEC;
+            const u32x4 zero = {0u, 0u, 0u, 0u};
+            const uint32_t chunk = r / VEC;
+            *reinterpret_cast<u32x4*>(to + O::row_at(row % VEC, chunk / 4u, row / VEC, chunk % 4u)) = r < a.rank ? staged[k] : zero;
+        }
+    };
+    V y[2][4];
+    auto column = [&](uint32_t i) {
+        const uint32_t n = first_column(i) + VEC * c;
         return n < a.N ? n : a.N - VEC;
     };
-    auto load = [&](Block& b, uint32_t i) __attribute__((always_inline)) {
+    auto request_y = [&](V (&to)[4], uint32_t i) __attribute__((always_inline)) {
+        if (LIVE && HAS_Y)
 #pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t row = column(i, u, lo >> 2) + (lo & 3u);
-#pragma unroll
-            for (uint32_t t = 0; t < NT; ++t)
-#pragma unroll
-                for (int f = 0; f < NF; ++f)
-                    b.m[u][t][f] = load16<V>(M + (uint64_t)(row + 4u * t) * a.rank + (r0[f] < a.rank ? r0[f] : 0u));
-            if (HAS_Y)
-#pragma unroll
-                for (int j = 0; j < SUB; ++j) b.y[u][j] = load16<V>(yr[j] + column(i, u, g));
-        }
+            for (int q = 0; q < 4; ++q) to[q] = LOADY(V, yr[q] + column(i));
     };
-    auto finish = [&](Block& b, uint32_t i) __attribute__((always_inline)) {
-        if (ragged)
+    auto compute = [&](const unsigned char* from, const V (&y)[4], uint32_t i) __attribute__((always_inline)) {
+        if (!LIVE) return;
+        const uint32_t base = first_column(i), col = column(i), cc = (col - base) / VEC;
+        f32x4 acc[VEC] = {};
 #pragma unroll
-            for (uint32_t u = 0; u < U; ++u)
+        for (int f = 0; f < NF; ++f)
 #pragma unroll
-                for (uint32_t t = 0; t < NT; ++t)
+            for (uint32_t t = 0; t < VEC; ++t) {
+                const V m = *reinterpret_cast<const V*>(from + O::row_at(t, f, cc, O::PAIR ? g & 1u : g));
 #pragma unroll
-                    for (int f = 0; f < NF; ++f) b.m[u][t][f] = r0[f] < a.rank ? b.m[u][t][f] : V{};
-#pragma unroll
-        for (int j = 0; j < SUB; ++j) {
-            f32x4 acc[U][NT] = {};
-#pragma unroll
-            for (int f = 0; f < NF; ++f)
-#pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    const V v = *reinterpret_cast<const V*>(lds + ((j * NF + f) * NP + p) * 1024u + lane * 16u);
-#pragma unroll
-                    for (uint32_t u = 0; u < U; ++u)
-#pragma unroll
-                        for (uint32_t t = 0; t < NT; ++t) acc[u][t] = X::mma(b.m[u][t][f], v, acc[u][t]);
-                }
-            const float d = X::SCALED ? down[16u * j + lo] : 1.0f;
-#pragma unroll
-            for (uint32_t u = 0; u < U; ++u) {
-                V o;
-#pragma unroll
-                for (uint32_t e = 0; e < VEC; ++e) {
-                    float v = acc[u][e / 4u][e % 4u];
-                    if (HAS_Y) v = X::SCALED ? __builtin_fmaf(v, d, (float)b.y[u][j][e]) : v + (float)b.y[u][j][e];
-                    else if (X::SCALED) v *= d;
-                    o[e] = (E)v;
-                }
-                __builtin_nontemporal_store(o, reinterpret_cast<V*>(outr[j] + column(i, u, g)));
+                for (int p = 0; p < NP; ++p) acc[t] = X::mma(vf[f][p], m, acc[t]);
             }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            V o;
+#pragma unroll
+            for (uint32_t t = 0; t < VEC; ++t) {
+                float v = acc[t][q];
+                if (HAS_Y) v = X::SCALED ? __builtin_fmaf(v, d[q], (float)y[q][t]) : v + (float)y[q][t];
+                else if (X::SCALED) v *= d[q];
+                o[t] = (E)v;
+            }
+            __builtin_nontemporal_store(o, reinterpret_cast<V*>(outr[q] + col));
         }
     };
-    if (!mine) return;
-    Block p, q;
+    auto meet = [&]() __attribute__((always_inline)) {
+        if (FEW) __builtin_amdgcn_wave_barrier();
+        else __syncthreads();
+    };
+    // block i from its buffer while block i + 1 comes in
+    auto advance = [&](const V (&now)[4], V (&next)[4], uint32_t i) __attribute__((always_inline)) {
+        request_rows(i + 1u);
+        request_y(next, i + 1u);
+        compute(buffer + (FEW ? 0u : (i & 1u) * O::BLOCK), now, i);
+        if (FEW) meet();
+        stage_rows(buffer + (FEW ? 0u : (i + 1u & 1u) * O::BLOCK));
+        meet();
+    };
+    request_rows(0);
+    request_y(y[0], 0);
+    stage_rows(buffer);
+    meet();
     uint32_t i = 0;
-    load(p, 0);
-    for (; i + 2u < mine; i += 2u) {
-        load(q, i + 1u);
-        finish(p, i);
-        load(p, i + 2u);
-        finish(q, i + 1u);
+    for (; i + 2u < blocks; i += 2u) {
+        advance(y[0], y[1], i);
+        advance(y[1], y[0], i + 1u);
     }
-    if (i + 1u < mine) {
-        load(q, i + 1u);
-        finish(p, i);
-        finish(q, i + 1u);
+    if (i + 1u < blocks) {
+        advance(y[0], y[1], i);
+        compute(buffer + (FEW ? 0u : O::BLOCK), y[1], i + 1u);
     } else {
-        finish(p, i);
+        compute(buffer, y[0], i);
     }
 }
 
 template <class E, int RT, bool HAS_Y, bool FEW>
-__global__ void __launch_bounds__(256, FEW || RT == 8 ? 1 : 2) expand_rows_kernel(ExpandArgs a)
+__global__ void __launch_bounds__(256, RT == 8 || FEW ? 1 : WE) expand_rows_kernel(ExpandArgs a)
 {
     using V = typename Mx<E>::V;
+    using O = Operand<E, RT>;
     constexpr uint32_t VEC = Mx<E>::VEC;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[Operand<E, RT>::BYTES];
-    __shared__ float down[64];
+    constexpr uint32_t buffers = (FEW ? 4u : 2u) * O::BLOCK;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[FEW && buffers < O::VECTORS ? O::VECTORS : buffers];
+    __shared__ float own_down[FEW ? 16 : 1];
     const PlanLayout L(a.tokens, a.n);
     Tile tile;
     uint32_t part;
     if (!take_tile<FEW>(a.plan, L, a.parts, tile, part)) return;
     if ((uint32_t)tile.adapter < a.n) {
-        make_operand<E, RT, FEW>(a, tile, lds, down, part == 0u);
-        if (a.N == 0u) return;
-        __syncthreads();
-        if constexpr (FEW) expand_tile<E, RT, 1, HAS_Y>(a, tile, part, lds, down);
-        else if (tile.count <= 32) expand_tile<E, RT, 2, HAS_Y>(a, tile, part, lds, down);
-        else expand_tile<E, RT, 4, HAS_Y>(a, tile, part, lds, down);
+        if constexpr (FEW) {
+            const uint32_t t = threadIdx.x >> 2, count = (uint32_t)tile.count;
+            if (t < 16u) {
+                const uint64_t position = (uint64_t)(uint32_t)tile.first + source_token(t, count);
+                f32x4 v[RT];
+                sum_parts<RT>(a.P, a.tokens, a.splits, position, v);
+                if (a.shrunk && part == 0u && t < count)
+                    store_shrunk<RT>(a.shrunk + (uint64_t)(uint32_t)a.plan[L.order + position] * a.rank, a.rank, v);
+                const float s = a.scales ? a.scales[tile.adapter] : 1.0f;
+#pragma unroll
+                for (int i = 0; i < RT; ++i) v[i] = v[i] * s;
+                const float d = store_vector<E, RT>(v, t, lds);
+                if (Mx<E>::SCALED && (threadIdx.x & 3u) == 0) own_down[t] = d;
+            }
+            __syncthreads();
+            expand_blocks<E, RT, HAS_Y, FEW, true>(a, tile, part, lds, lds, own_down);
+        } else {
+            const uint64_t id = blockIdx.x / a.parts;
+            const unsigned char* vectors = a.vectors + id * O::VECTORS;
+            // every wavefront meets the same barriers on either way
+            if (16u * this_wave() < (uint32_t)tile.count) expand_blocks<E, RT, HAS_Y, FEW, true>(a, tile, part, lds, vectors, a.down + id * 64u);
+            else expand_blocks<E, RT, HAS_Y, FEW, false>(a, tile, part, lds, vectors, a.down + id * 64u);
+        }
         return;
     }
     // tokens without an adapter: y as it is, or zeros
-    const uint32_t n0 = part * a.part;
-    const uint32_t n1 = a.N - n0 < a.part ? a.N : n0 + a.part;
-    if (a.N && (!HAS_Y || a.y.p != a.out))
+    if (!HAS_Y || a.y.p != a.out)
         for (uint32_t i = threadIdx.x >> 6; i < (uint32_t)tile.count; i += 4u) {
             const uint64_t t = (uint64_t)(uint32_t)a.plan[L.order + (uint32_t)tile.first + i];
-            for (uint32_t c = n0 + VEC * (threadIdx.x & 63u); c < n1; c += VEC * 64u) {
+            for (uint32_t c = VEC * (64u * part + (threadIdx.x & 63u)); c < a.N; c += VEC * 64u * a.parts) {
                 V v = {};
                 if (HAS_Y) v = load16<V>(static_cast<const E*>(a.y.p) + t * a.y.stride + c);
-                *reinterpret_cast<V*>(static_cast<E*>(a.out) + t * a.out_stride + c) = v;
+                __builtin_nontemporal_store(v, reinterpret_cast<V*>(static_cast<E*>(a.out) + t * a.out_stride + c));
             }
         }
-    if (a.shrunk && part == 0u)
+    if (FEW && a.shrunk && part == 0u)
         for (uint32_t i = threadIdx.x; i < (uint32_t)tile.count * a.rank; i += kThreads) {
             const uint32_t at = i / a.rank;
             a.shrunk[(uint64_t)(uint32_t)a.plan[L.order + (uint32_t)tile.first + at] * a.rank + (i - at * a.rank)] = 0.0f;
@@ -524,74 +698,14 @@ __global__ void __launch_bounds__(256) transpose_kernel(TransposeArgs a)
 }
 
 // ------------------------------------------------------------------------------------------------
-struct PiecesArgs {
-    const int32_t* plan;
-    const float* P;       // d / s: [splits][tokens][16 RT]
-    const float* shrunk;  // u: [tokens][rank]
-    const float* scales;
-    void* pieces[2];      // d, s u: [tiles][16 RT][PIECES][64]
-    float* down;          // fp16: [2][tiles], the inverse of the tile's scaling
-    uint64_t tokens, max_tiles;
-    uint32_t n, rank, rp, splits;
-};
-
-// Transposes a tile's d (or s u) and splits it.  Tokens behind the tile's count and ranks behind the
-// adapter's are zeros.
-template <class E>
-__global__ void __launch_bounds__(256) weight_pieces_kernel(PiecesArgs a)
-{
-    using X = Mx<E>;
-    __shared__ float top[4];
-    const PlanLayout L(a.tokens, a.n);
-    if (blockIdx.x >= (uint32_t)a.plan[L.counts]) return;
-    const Tile tile = reinterpret_cast<const Tile*>(a.plan)[blockIdx.x];
-    if ((uint32_t)tile.adapter >= a.n) return;
-    const uint32_t which = blockIdx.y, lane = threadIdx.x & 63u, wave = this_wave();
-    const float s = a.scales ? a.scales[tile.adapter] : 1.0f;
-    const bool live = lane < (uint32_t)tile.count;
-    const uint64_t pos = (uint64_t)(uint32_t)tile.first + lane;
-    const int64_t token = live ? a.plan[L.order + pos] : 0;
-    auto value = [&](uint32_t r) {
-        if (!live || r >= a.rank) return 0.0f;
-        if (which) return a.shrunk[token * a.rank + r] * s;
-        float sum = 0.0f;
-        for (uint32_t sp = 0; sp < a.splits; ++sp) sum += a.P[((uint64_t)sp * a.tokens + pos) * a.rp + r];
-        return sum * s;
-    };
-    float up = 1.0f;
-    if constexpr (X::SCALED) {
-        float m = 0.0f, down;
-        for (uint32_t r = wave; r < a.rp; r += 4u) m = fmaxf(m, finite_magnitude(value(r)));
-        for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-        if (lane == 0) top[wave] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        half_scale(m, up, down);
-        if (threadIdx.x == 0) a.down[which * a.max_tiles + blockIdx.x] = down;
-    }
-    E* out = static_cast<E*>(a.pieces[which]) + (uint64_t)blockIdx.x * a.rp * X::PIECES * 64u;
-    for (uint32_t r = wave; r < a.rp; r += 4u) {
-        const float v = value(r) * up;
-        if constexpr (X::PIECES == 1) {
-            out[r * 64u + lane] = v;
-        } else {
-            E hi, low;
-            split<E>(v, hi, low);
-            out[(2u * r) * 64u + lane] = hi;
-            out[(2u * r + 1u) * 64u + lane] = low;
-        }
-    }
-}
-
-// ------------------------------------------------------------------------------------------------
 struct WeightArgs {
     const int32_t* plan;
     Rows rows[2];         // x, dy
     const void* pieces[2];
-    const float* down;
+    const float* down[2]; // fp16: [tiles], the inverse of the pieces' scaling
     float* partials;      // [slots][rank * (K + N)]
     void* grad[2];        // dA [n][rank][K], dB [n][N][rank]
-    uint64_t tokens, max_tiles;
+    uint64_t tokens;
     uint32_t n, rank, rp, len[2];
     uint32_t blocks0;     // workgroups along K
 };
@@ -659,7 +773,7 @@ __global__ void __launch_bounds__(256) weight_rows_kernel(WeightArgs a)
                 wf[j][p] = load16<V>(pieces + (((uint64_t)tile * a.rp + rank0 + 16u * j + lo) * X::PIECES + p) * 64u + t0 % kTile + VEC * g);
         turn_over(in, turned);
         if constexpr (X::SCALED) {
-            const float down = a.down[which * a.max_tiles + tile];
+            const float down = a.down[which][tile];
 #pragma unroll
             for (int j = 0; j < RT; ++j)
 #pragma unroll
@@ -772,25 +886,24 @@ __global__ void __launch_bounds__(256) weight_sum_kernel(WeightSumArgs a)
 // ------------------------------------------------------------------------------------------------
 uint32_t padded_rank(uint32_t rank) { return rank <= 16u ? 16u : rank <= 32u ? 32u : rank <= 64u ? 64u : 128u; }
 
-// How an axis is cut: `most` workgroups or a little fewer, but no part smaller than a unit; where there are eight
-// parts or more, a multiple of eight, one XCD's share each.
-void cut(uint64_t tiles, uint32_t length, uint32_t unit, uint32_t most, uint32_t& part, uint32_t& parts)
+// How many workgroups share the blocks of an axis: so many that there are `most` in all, each with at least
+// `least` blocks; eight, one for each XCD, or a multiple of eight where the blocks allow it.
+uint32_t cut(uint64_t tiles, uint32_t blocks, uint32_t least, uint32_t most)
 {
-    const uint32_t units = (length + unit - 1u) / unit;
-    uint64_t want = tiles && units ? most / tiles : 1u;
-    if (want < 1u) want = 1u;
-    if (want > units) want = units ? units : 1u;
-    if (want > 8u) want = want / 8u * 8u;
-    part = (units + (uint32_t)want - 1u) / (uint32_t)want * unit;
-    if (!part) part = unit;
-    parts = length ? (length + part - 1u) / part : 1u;
+    uint32_t parts = (uint32_t)(tiles && most / tiles > 8u ? most / tiles : 8u);
+    const uint32_t limit = blocks / least ? blocks / least : 1u;
+    if (parts > limit) parts = limit;
+    return parts > 8u ? parts / 8u * 8u : parts;
 }
 
+#ifndef EB
+#define EB 2u
+#endif
 #ifndef MC
-#define MC 512u
+#define MC 1024u
 #endif
 #ifndef ME
-#define ME 1024u
+#define ME 2048u
 #endif
 template <class F>
 void for_rank(uint32_t rp, F f)
@@ -804,7 +917,6 @@ void for_rank(uint32_t rp, F f)
 }
 
 uint32_t elements_of(int dtype) { return dtype == MI_F32 ? 4u : 8u; }
-uint64_t up256(uint64_t bytes) { return (bytes + 255u) / 256u * 256u; }
 
 int check(const mi_lora* d)
 {
@@ -818,74 +930,128 @@ int check(const mi_lora* d)
     return MI_OK;
 }
 
-// How a batch is cut, and the forward pass's workspace: the partial sums P.  With few tokens for each adapter
-// (16 on the average, or 256 in all) workgroups take 16 tokens instead of 64: a fourth of the registers, so
-// that four times as many wavefronts hide the latencies that such a batch consists of.
-struct ForwardPlan {
+// How a batch is cut.  With few tokens for each adapter (16 on the average, or 256 in all) workgroups take 16
+// tokens instead of 64, and their wavefronts different parts of the adapter, which is then most of what
+// there is to read; and the expansion adds up the parts of P itself, a launch less.
+struct Cut {
     bool few;
-    uint32_t rp, part, splits, npart, nparts;
-    uint64_t tiles, bytes;  // tiles: that the grids provide for, absent ones among them
-    ForwardPlan(const mi_lora* d, uint32_t K, uint32_t N)
+    uint32_t rp, splits, parts;
+    uint64_t max_tiles, grid_tiles;  // of the plan; that the grids provide for
+    Cut(const mi_lora* d, uint32_t K, uint32_t N)
     {
-        const PlanLayout L(d->tokens, d->n_adapters);
+        max_tiles = PlanLayout(d->tokens, d->n_adapters).max_tiles;
         few = d->tokens <= 256u || d->tokens <= 16u * d->n_adapters;
-        tiles = L.max_tiles;
+        grid_tiles = few ? 4u * max_tiles : max_tiles;
         rp = padded_rank(d->rank);
-        const uint32_t step = 4u * elements_of(d->dtype);
-        cut(tiles, K, 8u * step, few ? 1024u : MC, part, splits);  // each wavefront two blocks of two steps at least
-        cut(tiles, N, 8u * step, few ? 1024u : ME, npart, nparts);  // each wavefront a 128-byte line at least
-        if (few) tiles *= 4u;
-        bytes = up256((uint64_t)splits * d->tokens * rp * 4u);
+        const uint32_t block = 16u * elements_of(d->dtype);  // columns of a block, of x and of y
+        splits = cut(max_tiles, (K + block - 1u) / block, few ? 4u : 2u, MC);
+        parts = cut(max_tiles, (N + block - 1u) / block, few ? 4u : EB, few ? 1024u : ME);
+    }
+    uint64_t sums() const { return (uint64_t)splits * rp * 4u; }  // bytes of P per token
+};
+
+struct Take {  // places in a workspace
+    uint64_t end = 0;
+    uint64_t operator()(uint64_t bytes)
+    {
+        const uint64_t here = end;
+        end += (bytes + 255u) / 256u * 256u;
+        return here;
+    }
+};
+
+uint64_t pieces_bytes(uint32_t rp) { return (uint64_t)rp * 64u * 4u; }  // two of 2 bytes, or one of 4
+
+struct ForwardPlan {
+    Cut c;
+    uint64_t P, vectors, down, bytes;
+    explicit ForwardPlan(const mi_lora* d) : c(d, d->K, d->N)
+    {
+        Take take;
+        P = take(c.sums() * d->tokens);
+        vectors = take(c.few ? 0u : c.max_tiles * pieces_bytes(c.rp));
+        down = take(c.few ? 0u : c.max_tiles * 64u * 4u);
+        bytes = take.end;
     }
 };
 
 struct BackwardPlan {
-    ForwardPlan f;  // contraction over N, expansion to K
-    ForwardPlan u;  // contraction over K alone, when the forward pass's sums are not given
-    uint64_t at, bt, shrunk, pieces[2], down, partials, bytes;
-    explicit BackwardPlan(const mi_lora* d) : f(d, d->N, d->K), u(d, d->K, 0u)
+    Cut c;  // contraction over N, expansion to K
+    Cut u;  // contraction over K as the forward pass does it, when its sums are not given
+    uint64_t P, at, bt, vectors, down, pieces[2], tile_down[2], partials, bytes;
+    explicit BackwardPlan(const mi_lora* d) : c(d, d->N, d->K), u(d, d->K, d->N)
     {
         const PlanLayout L(d->tokens, d->n_adapters);
-        const uint64_t e = d->dtype == MI_F32 ? 4u : 2u, pieces_n = d->dtype == MI_F32 ? 1u : 2u;
-        uint64_t at_ = f.bytes > u.bytes ? f.bytes : u.bytes;  // P first, in turn
-        auto take = [&](uint64_t n) { const uint64_t here = at_; at_ += up256(n); return here; };
+        const uint64_t e = d->dtype == MI_F32 ? 4u : 2u;
+        c.few = false;
+        c.grid_tiles = c.max_tiles;
+        Take take;
+        P = take((c.sums() > u.sums() ? c.sums() : u.sums()) * d->tokens);  // in turn
         at = take((uint64_t)d->n_adapters * d->rank * d->K * e);
         bt = take((uint64_t)d->n_adapters * d->rank * d->N * e);
-        shrunk = take(d->tokens * d->rank * 4u);
-        for (int i = 0; i < 2; ++i) pieces[i] = take(L.max_tiles * f.rp * pieces_n * 64u * e);
-        down = take(2u * L.max_tiles * 4u);
+        vectors = take(c.max_tiles * pieces_bytes(c.rp));
+        down = take(c.max_tiles * 64u * 4u);
+        for (int i = 0; i < 2; ++i) {
+            pieces[i] = take(c.max_tiles * pieces_bytes(c.rp));
+            tile_down[i] = take(c.max_tiles * 4u);
+        }
         partials = take(L.max_slots * d->rank * ((uint64_t)d->K + d->N) * 4u);
-        bytes = at_;
+        bytes = take.end;
     }
 };
 
 template <class E>
-int contract(const mi_lora* d, const int32_t* plan, Rows x, const void* M, uint32_t K, const ForwardPlan& f, float* P, hipStream_t s)
+int contract(const mi_lora* d, const int32_t* plan, Rows x, const void* M, uint32_t K, const Cut& c, float* P, hipStream_t s)
 {
-    ContractArgs a{plan, x, M, P, d->tokens, d->n_adapters, d->rank, K, f.splits, f.part};
-    for_rank(f.rp, [&](auto rt) {
+    ContractArgs a{plan, x, M, P, d->tokens, d->n_adapters, d->rank, K, c.splits};
+    const dim3 grid((uint32_t)c.grid_tiles * c.splits);
+    for_rank(c.rp, [&](auto rt) {
         constexpr int RT = decltype(rt)::value;
-        const dim3 grid((uint32_t)f.tiles * f.splits);
-        if (f.few) hipLaunchKernelGGL((contract_rows_kernel<E, RT, true>), grid, dim3(kThreads), 0, s, a);
+        if (c.few) hipLaunchKernelGGL((contract_rows_kernel<E, RT, true>), grid, dim3(kThreads), 0, s, a);
         else hipLaunchKernelGGL((contract_rows_kernel<E, RT, false>), grid, dim3(kThreads), 0, s, a);
     });
     return launch_status();
 }
 
 template <class E>
-int expand(const mi_lora* d, const int32_t* plan, Rows y, void* out, uint64_t out_stride, const void* M, uint32_t N, const float* scales,
-           const ForwardPlan& f, const float* P, float* shrunk, hipStream_t s)
+int tile_vectors(const Cut& c, const VectorArgs& a, hipStream_t s)
 {
-    ExpandArgs a{plan, y, out, out_stride, M, scales, P, shrunk, d->tokens, d->n_adapters, d->rank, N, f.splits, f.npart, f.nparts};
-    const dim3 grid((uint32_t)f.tiles * f.nparts);
-    for_rank(f.rp, [&](auto rt) {
+    for_rank(c.rp, [&](auto rt) {
+        hipLaunchKernelGGL((tile_vectors_kernel<E, decltype(rt)::value>), dim3((uint32_t)c.max_tiles), dim3(kThreads), 0, s, a);
+    });
+    return launch_status();
+}
+
+template <class E>
+int expand(const Cut& c, ExpandArgs a, hipStream_t s)
+{
+    a.parts = c.parts;
+    a.splits = c.splits;
+    const dim3 grid((uint32_t)c.grid_tiles * c.parts);
+    for_rank(c.rp, [&](auto rt) {
         constexpr int RT = decltype(rt)::value;
-        if (y.p && f.few) hipLaunchKernelGGL((expand_rows_kernel<E, RT, true, true>), grid, dim3(kThreads), 0, s, a);
-        else if (y.p) hipLaunchKernelGGL((expand_rows_kernel<E, RT, true, false>), grid, dim3(kThreads), 0, s, a);
-        else if (f.few) hipLaunchKernelGGL((expand_rows_kernel<E, RT, false, true>), grid, dim3(kThreads), 0, s, a);
+        if (a.y.p && c.few) hipLaunchKernelGGL((expand_rows_kernel<E, RT, true, true>), grid, dim3(kThreads), 0, s, a);
+        else if (a.y.p) hipLaunchKernelGGL((expand_rows_kernel<E, RT, true, false>), grid, dim3(kThreads), 0, s, a);
         else hipLaunchKernelGGL((expand_rows_kernel<E, RT, false, false>), grid, dim3(kThreads), 0, s, a);
     });
     return launch_status();
+}
+
+template <class E>
+int forward(const mi_lora* d, const void* y, const void* x, const void* A, const void* B, const float* scales, const int32_t* plan, void* out,
+            float* shrunk, unsigned char* ws, hipStream_t s)
+{
+    const ForwardPlan f(d);
+    float* P = reinterpret_cast<float*>(ws + f.P);
+    float* down = reinterpret_cast<float*>(ws + f.down);
+    int st;
+    if ((st = contract<E>(d, plan, {x, d->x_stride}, A, d->K, f.c, P, s)) != MI_OK) return st;
+    if (!f.c.few) {
+        const VectorArgs v{plan, P, scales, shrunk, ws + f.vectors, down, nullptr, nullptr, d->tokens, d->n_adapters, d->rank, f.c.splits, false};
+        if ((st = tile_vectors<E>(f.c, v, s)) != MI_OK) return st;
+    }
+    return expand<E>(f.c, {plan, {y, d->y_stride}, out, d->out_stride, B, ws + f.vectors, down, scales, P, shrunk, d->tokens, d->n_adapters,
+                           d->rank, d->N, 0, 0}, s);
 }
 
 template <class E>
@@ -893,42 +1059,46 @@ int backward(const mi_lora* d, const void* dy, const void* x, const void* A, con
              const float* shrunk, const void* dx_in, void* dx, void* dA, void* dB, unsigned char* ws, hipStream_t s)
 {
     const BackwardPlan b(d);
-    float* P = reinterpret_cast<float*>(ws);
+    float* P = reinterpret_cast<float*>(ws + b.P);
+    float* down = reinterpret_cast<float*>(ws + b.down);
+    float* tile_down[2] = {reinterpret_cast<float*>(ws + b.tile_down[0]), reinterpret_cast<float*>(ws + b.tile_down[1])};
     const Rows rx{x, d->x_stride}, rdy{dy, d->y_stride};
     int st;
-    if (d->tokens == 0) {
-        WeightSumArgs w{plan, P, {dA, dB}, 0, d->n_adapters, d->rank, {d->K, d->N}};
-        hipLaunchKernelGGL((weight_sum_kernel<E>), dim3(64, d->n_adapters), dim3(kThreads), 0, s, w);
-        return launch_status();
+    if (d->tokens) {
+        // s u, transposed
+        VectorArgs v{plan, P, scales, const_cast<float*>(shrunk), nullptr, nullptr, ws + b.pieces[1], tile_down[1],
+                     d->tokens, d->n_adapters, d->rank, b.u.splits, shrunk != nullptr};
+        if (!shrunk && (st = contract<E>(d, plan, rx, A, d->K, b.u, P, s)) != MI_OK) return st;
+        if ((st = tile_vectors<E>(b.c, v, s)) != MI_OK) return st;
+        // d, both ways
+        const uint32_t across = (d->rank + 63u) / 64u;
+        TransposeArgs t{plan, {A, B}, {ws + b.at, ws + b.bt}, d->tokens, d->n_adapters, {d->rank, d->N}, {d->K, d->rank}, across * ((d->K + 63u) / 64u)};
+        hipLaunchKernelGGL((transpose_kernel<E>), dim3(t.blocks0 + across * ((d->N + 63u) / 64u), d->n_adapters), dim3(kThreads), 0, s, t);
+        if ((st = launch_status()) != MI_OK) return st;
+        if ((st = contract<E>(d, plan, rdy, ws + b.bt, d->N, b.c, P, s)) != MI_OK) return st;
+        v.shrunk = nullptr;
+        v.given = false;
+        v.splits = b.c.splits;
+        v.vectors = ws + b.vectors;
+        v.down = down;
+        v.pieces = ws + b.pieces[0];
+        v.tile_down = tile_down[0];
+        if ((st = tile_vectors<E>(b.c, v, s)) != MI_OK) return st;
+        if ((st = expand<E>(b.c, {plan, {dx_in, d->out_stride}, dx, d->out_stride, ws + b.at, ws + b.vectors, down, nullptr, nullptr, nullptr,
+                                  d->tokens, d->n_adapters, d->rank, d->K, 0, 0}, s)) != MI_OK)
+            return st;
+        const PlanLayout L(d->tokens, d->n_adapters);
+        const uint32_t cols = 16u * Mx<E>::VEC, blocks0 = (d->K + cols - 1u) / cols, blocks1 = (d->N + cols - 1u) / cols;
+        WeightArgs w{plan, {rx, rdy}, {ws + b.pieces[0], ws + b.pieces[1]}, {tile_down[0], tile_down[1]}, reinterpret_cast<float*>(ws + b.partials),
+                     {dA, dB}, d->tokens, d->n_adapters, d->rank, b.c.rp, {d->K, d->N}, blocks0};
+        const uint32_t rt = b.c.rp <= 64u ? b.c.rp : 64u;
+        const dim3 grid(blocks0 + blocks1, (uint32_t)L.max_chunks, b.c.rp / rt);
+        if (rt == 16u) hipLaunchKernelGGL((weight_rows_kernel<E, 1>), grid, dim3(kThreads), 0, s, w);
+        else if (rt == 32u) hipLaunchKernelGGL((weight_rows_kernel<E, 2>), grid, dim3(kThreads), 0, s, w);
+        else hipLaunchKernelGGL((weight_rows_kernel<E, 4>), grid, dim3(kThreads), 0, s, w);
+        if ((st = launch_status()) != MI_OK) return st;
     }
-    if (!shrunk) {  // u again
-        if ((st = contract<E>(d, plan, rx, A, d->K, b.u, P, s)) != MI_OK) return st;
-        float* u = reinterpret_cast<float*>(ws + b.shrunk);
-        // the sums into the tokens' order: an expansion to no columns
-        if ((st = expand<E>(d, plan, {nullptr, 0}, nullptr, 0, A, 0, nullptr, b.u, P, u, s)) != MI_OK) return st;
-        shrunk = u;
-    }
-    const uint32_t across = (d->rank + 63u) / 64u;
-    TransposeArgs t{plan, {A, B}, {ws + b.at, ws + b.bt}, d->tokens, d->n_adapters, {d->rank, d->N}, {d->K, d->rank}, across * ((d->K + 63u) / 64u)};
-    hipLaunchKernelGGL((transpose_kernel<E>), dim3(t.blocks0 + across * ((d->N + 63u) / 64u), d->n_adapters), dim3(kThreads), 0, s, t);
-    if ((st = launch_status()) != MI_OK) return st;
-    if ((st = contract<E>(d, plan, rdy, ws + b.bt, d->N, b.f, P, s)) != MI_OK) return st;
-    if ((st = expand<E>(d, plan, {dx_in, d->out_stride}, dx, d->out_stride, ws + b.at, d->K, scales, b.f, P, nullptr, s)) != MI_OK) return st;
-    const PlanLayout L(d->tokens, d->n_adapters);
-    PiecesArgs p{plan, P, shrunk, scales, {ws + b.pieces[0], ws + b.pieces[1]}, reinterpret_cast<float*>(ws + b.down),
-                 d->tokens, L.max_tiles, d->n_adapters, d->rank, b.f.rp, b.f.splits};
-    hipLaunchKernelGGL((weight_pieces_kernel<E>), dim3((uint32_t)L.max_tiles, 2), dim3(kThreads), 0, s, p);
-    if ((st = launch_status()) != MI_OK) return st;
-    const uint32_t cols = 16u * Mx<E>::VEC, blocks0 = (d->K + cols - 1u) / cols, blocks1 = (d->N + cols - 1u) / cols;
-    WeightArgs w{plan, {rx, rdy}, {p.pieces[0], p.pieces[1]}, p.down, reinterpret_cast<float*>(ws + b.partials), {dA, dB},
-                 d->tokens, L.max_tiles, d->n_adapters, d->rank, b.f.rp, {d->K, d->N}, blocks0};
-    const uint32_t rt = b.f.rp <= 64u ? b.f.rp : 64u;
-    const dim3 grid(blocks0 + blocks1, (uint32_t)L.max_chunks, b.f.rp / rt);
-    if (rt == 16u) hipLaunchKernelGGL((weight_rows_kernel<E, 1>), grid, dim3(kThreads), 0, s, w);
-    else if (rt == 32u) hipLaunchKernelGGL((weight_rows_kernel<E, 2>), grid, dim3(kThreads), 0, s, w);
-    else hipLaunchKernelGGL((weight_rows_kernel<E, 4>), grid, dim3(kThreads), 0, s, w);
-    if ((st = launch_status()) != MI_OK) return st;
-    WeightSumArgs sum{plan, w.partials, {dA, dB}, d->tokens, d->n_adapters, d->rank, {d->K, d->N}};
+    WeightSumArgs sum{plan, reinterpret_cast<float*>(ws + b.partials), {dA, dB}, d->tokens, d->n_adapters, d->rank, {d->K, d->N}};
     hipLaunchKernelGGL((weight_sum_kernel<E>), dim3(64, d->n_adapters), dim3(kThreads), 0, s, sum);
     return launch_status();
 }
@@ -941,7 +1111,7 @@ extern "C" uint64_t mi_lora_workspace(const mi_lora* d, int backward)
 {
     using namespace mi::adapters;
     if (check(d) != MI_OK) return 0;
-    return backward ? BackwardPlan(d).bytes : ForwardPlan(d, d->K, d->N).bytes;
+    return backward ? BackwardPlan(d).bytes : ForwardPlan(d).bytes;
 }
 
 extern "C" int mi_lora_add(const void* y, const void* x, const void* A, const void* B, const float* scales, const int32_t* plan, void* out,
@@ -956,16 +1126,11 @@ extern "C" int mi_lora_add(const void* y, const void* x, const void* A, const vo
         reinterpret_cast<uintptr_t>(scales) & 3u || reinterpret_cast<uintptr_t>(shrunk) & 3u)
         return MI_ERR_ALIGN;
     if (y == out && d->y_stride != d->out_stride && d->tokens > 1u) return MI_ERR_ALIAS;
-    const ForwardPlan f(d, d->K, d->N);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    float* P = static_cast<float*>(workspace);
-    auto both = [&](auto e) {
-        using E = decltype(e);
-        const int first = contract<E>(d, plan, {x, d->x_stride}, A, d->K, f, P, s);
-        return first != MI_OK ? first
-                              : expand<E>(d, plan, {y, d->y_stride}, out, d->out_stride, B, d->N, scales, f, P, shrunk, s);
-    };
-    return d->dtype == MI_F32 ? both(float{}) : d->dtype == MI_BF16 ? both(__bf16{}) : both(_Float16{});
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    if (d->dtype == MI_F32) return forward<float>(d, y, x, A, B, scales, plan, out, shrunk, ws, s);
+    if (d->dtype == MI_BF16) return forward<__bf16>(d, y, x, A, B, scales, plan, out, shrunk, ws, s);
+    return forward<_Float16>(d, y, x, A, B, scales, plan, out, shrunk, ws, s);
 }
 
 extern "C" int mi_lora_add_backward(const void* dy, const void* x, const void* A, const void* B, const float* scales, const int32_t* plan,
