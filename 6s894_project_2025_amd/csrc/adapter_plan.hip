@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const Id* ids, uint3
                 hist[w * keys + k] = total;
                 total += c;
             }
-        const uint32_t chunks = k < n ? (total + kChunk - 1u) / kChunk : 0u;
+        const uint32_t chunks = k < n ? (total + L.chunk - 1u) / L.chunk : 0u;
         const uint32_t add[4] = {total, (total + kTile - 1u) / kTile, chunks, chunks > 1u ? chunks : 0u};
         uint32_t* out[4] = {start, tile_start, chunk_start, slot_start};
         for (int i = 0; i < 4; ++i) {
@@ -128,11 +128,11 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const Id* ids, uint3
     }
     Chunk* chunks = reinterpret_cast<Chunk*>(plan + L.chunks);
     for (uint32_t i = threadIdx.x; i < chunk_start[keys]; i += kThreads) {
-        const uint32_t k = owner(chunk_start, i), c = i - chunk_start[k], first = start[k] + c * kChunk;
+        const uint32_t k = owner(chunk_start, i), c = i - chunk_start[k], first = start[k] + c * L.chunk;
         const uint32_t left = start[k + 1u] - first;
         const bool many = slot_start[k + 1u] > slot_start[k];
-        chunks[i] = Chunk{(int32_t)k, (int32_t)first, (int32_t)(left < kChunk ? left : kChunk),
-                          many ? (int32_t)(slot_start[k] + c) : -1, (int32_t)(tile_start[k] + c * (kChunk / kTile)), {0, 0, 0}};
+        chunks[i] = Chunk{(int32_t)k, (int32_t)first, (int32_t)(left < L.chunk ? left : L.chunk),
+                          many ? (int32_t)(slot_start[k] + c) : -1, (int32_t)(tile_start[k] + c * (L.chunk / kTile)), {0, 0, 0}};
     }
 }
 

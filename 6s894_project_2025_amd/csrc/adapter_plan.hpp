@@ -8,7 +8,7 @@ namespace mi {
 namespace adapters {
 
 constexpr uint32_t kTile = 64;        // tokens of one adapter that a workgroup takes together
-constexpr uint32_t kChunk = 512;      // tokens of one adapter behind one partial weight gradient
+constexpr uint32_t kMaxChunk = 512;
 constexpr uint32_t kMaxAdapters = 1024;
 // A grid has at most 65535 workgroups along its second axis, where chunks and parts of K or N are.
 constexpr uint64_t kMaxTokens = 1u << 24;
@@ -22,6 +22,7 @@ struct Chunk {  // slot: row of partial sums, or -1 where the adapter has no oth
 };
 
 struct PlanLayout {
+    uint32_t chunk;  // tokens of one adapter behind one partial weight gradient: few where there are few to share out
     uint64_t max_tiles, max_chunks, max_slots;
     uint64_t chunks, counts, slot_start, order, starts, size;  // offsets in int32; tiles are at 0
 
@@ -29,10 +30,11 @@ struct PlanLayout {
     {
         const uint64_t groups = tokens < n + 1ull ? tokens : n + 1ull;  // at most so many are not empty
         max_tiles = tokens / kTile + groups;
-        max_chunks = tokens / kChunk + groups;
-        // only adapters with more than kChunk tokens have slots: at most tokens / kChunk of them, and
-        // ceil(c / kChunk) <= 2 c / kChunk for each
-        max_slots = 2u * (tokens / kChunk);
+        chunk = tokens < 4096u ? 128u : 512u;
+        max_chunks = tokens / chunk + groups;
+        // only adapters with more than `chunk` tokens have slots: at most tokens / chunk of them, and
+        // ceil(c / chunk) <= 2 c / chunk for each
+        max_slots = 2u * (tokens / chunk);
         chunks = 4u * max_tiles;
         counts = chunks + 8u * max_chunks;  // {tiles, chunks}
         slot_start = counts + 2u;           // [n]

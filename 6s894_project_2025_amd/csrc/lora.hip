@@ -13,10 +13,10 @@
 // Tokens come grouped by adapter (adapter_plan.hpp), in tiles of up to 64 of one adapter.
 //   contract_rows   P[split][position][r] = sum over a part of the long axis of row . M[a]:  u, and d / s
 //   expand_rows     out = y + s (sum of P) M'[a]^T:  the forward output, and dx
-//   transpose       B^T and A^T of the adapters in use, which give the backward pass the layouts of the
-//                   forward one
+//   gradient_rows   dB of up to 512 tokens and P of d, from one pass over g
+//   transpose       A^T of the adapters in use, for dx by expand_rows
 //   tile_vectors    the sums of P times s, split, as operands of expand_rows and, transposed, of weight_rows
-//   weight_rows     dA and dB of up to 512 tokens;  weight_sum adds these up
+//   weight_rows     dA of up to 512 tokens;  weight_sum adds the weights' parts up
 // All sums are in a fixed order.
 #include <type_traits>
 
@@ -669,45 +669,42 @@ __global__ void __launch_bounds__(256, RT == 8 || FEW ? 1 : WE) expand_rows_kern
 // ------------------------------------------------------------------------------------------------
 struct TransposeArgs {
     const int32_t* plan;
-    const void* src[2];  // A [n][rank][K], B [n][N][rank]
-    void* dst[2];        // [n][K][rank], [n][rank][N]
+    const void* src;     // A [n][rank][K]
+    void* dst;           // [n][K][rank]
     uint64_t tokens;
-    uint32_t n, rows[2], cols[2];
-    uint32_t blocks0;    // workgroups of the first matrix
+    uint32_t n, rank, K;
 };
 
-// 64 x 64 pieces of the adapters in use.
+// A^T of the adapters in use: a thread has eight ranks of one k, so that reads are whole lines along k and the
+// stores 16 or 32 bytes of the neighbouring rows.
 template <class E>
 __global__ void __launch_bounds__(256) transpose_kernel(TransposeArgs a)
 {
-    __shared__ E tile[64][66];
     const PlanLayout L(a.tokens, a.n);
-    const uint32_t ad = blockIdx.y;
-    if (a.plan[L.starts + ad] == a.plan[L.starts + ad + 1u]) return;
-    const uint32_t which = blockIdx.x >= a.blocks0;
-    const uint32_t b = blockIdx.x - which * a.blocks0, rows = a.rows[which], cols = a.cols[which];
-    const uint32_t across = (cols + 63u) / 64u, r0 = b / across * 64u, c0 = b % across * 64u;
-    const E* src = static_cast<const E*>(a.src[which]) + (uint64_t)ad * rows * cols;
-    E* dst = static_cast<E*>(a.dst[which]) + (uint64_t)ad * rows * cols;
-    const uint32_t x = threadIdx.x & 63u, y0 = threadIdx.x >> 6;
-    for (uint32_t y = y0; y < 64u; y += 4u)
-        if (r0 + y < rows && c0 + x < cols) tile[y][x] = src[(uint64_t)(r0 + y) * cols + c0 + x];
-    __syncthreads();
-    for (uint32_t y = y0; y < 64u; y += 4u)
-        if (c0 + y < cols && r0 + x < rows) dst[(uint64_t)(c0 + y) * rows + r0 + x] = tile[x][y];
+    const uint32_t k = blockIdx.x * kThreads + threadIdx.x, r0 = 8u * blockIdx.y, ad = blockIdx.z;
+    if (k >= a.K || a.plan[L.starts + ad] == a.plan[L.starts + ad + 1u]) return;
+    const E* src = static_cast<const E*>(a.src) + ((uint64_t)ad * a.rank + r0) * a.K + k;
+    typedef E E4 __attribute__((ext_vector_type(4)));
+    E4 v[2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = src[(uint64_t)i * a.K];
+    E4* dst = reinterpret_cast<E4*>(static_cast<E*>(a.dst) + ((uint64_t)ad * a.K + k) * a.rank + r0);
+    dst[0] = v[0];
+    dst[1] = v[1];
 }
 
 // ------------------------------------------------------------------------------------------------
 struct WeightArgs {
     const int32_t* plan;
-    Rows rows[2];         // x, dy
-    const void* pieces[2];
-    const float* down[2]; // fp16: [tiles], the inverse of the pieces' scaling
+    Rows rows;            // x, dy
+    const void* pieces;
+    const float* down;    // fp16: [tiles], the inverse of the pieces' scaling
     float* partials;      // [slots][rank * (K + N)]
-    void* grad[2];        // dA [n][rank][K], dB [n][N][rank]
+    void* grad;           // dA [n][rank][K], dB [n][N][rank]
+    const void* B;        // [n][N][rank], with dy
+    float* P;             // [slices][tokens][rp], with dy: d / s by slices of N
     uint64_t tokens;
-    uint32_t n, rank, rp, len[2];
-    uint32_t blocks0;     // workgroups along K
+    uint32_t n, rank, rp, K, N;
 };
 
 // Four 16-byte rows' registers to fragments along the tokens: in[i] holds VEC consecutive columns of
@@ -728,105 +725,69 @@ __device__ __forceinline__ void turn_over(const u32x4 (&in)[4], u32x4 (&out)[4])
         for (int p = 0; p < 4; ++p) out[c][p] = in[p][c];
 }
 
-// Workgroup: a chunk of up to 512 tokens of one adapter, 16 VEC columns, up to RT * 16 ranks.  A wavefront
-// takes every fourth step of STEP tokens; a lane reads 16 bytes of VEC consecutive tokens (the 16 lanes of a
-// group read 256 contiguous bytes of a row) and turns them over in registers, one byte permute for two
-// values, so the contraction over tokens needs no LDS.  The wavefronts' sums meet in LDS at the end.
+// One step of the contraction over tokens: acc[j][c] += pieces of 16 ranks (rows) . column VEC lo + c.
 template <class E, int RT>
-__global__ void __launch_bounds__(256) weight_rows_kernel(WeightArgs a)
+__device__ __forceinline__ void weight_step(const WeightArgs& a, uint32_t tile, uint32_t t0, uint32_t rank0, const u32x4 (&in)[Mx<E>::VEC],
+                                            f32x4 (&acc)[RT][Mx<E>::VEC])
 {
     using X = Mx<E>;
     using V = typename X::V;
-    constexpr uint32_t VEC = X::VEC, STEP = X::STEP;
-    __shared__ f32x4 red[2 * RT * VEC * 64];
-    __shared__ int32_t order[kChunk];
-    const PlanLayout L(a.tokens, a.n);
-    if (blockIdx.y >= (uint32_t)a.plan[L.counts + 1u]) return;
-    const Chunk chunk = reinterpret_cast<const Chunk*>(a.plan + L.chunks)[blockIdx.y];
-    const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), lo = lane & 15u, g = lane >> 4;
-    for (uint32_t i = threadIdx.x; i < (uint32_t)chunk.count; i += kThreads)
-        order[i] = a.plan[L.order + (uint32_t)chunk.first + i];
-    __syncthreads();
-    const uint32_t which = blockIdx.x >= a.blocks0;
-    const uint32_t len = a.len[which], col = (blockIdx.x - which * a.blocks0) * 16u * VEC + VEC * lo;
-    const uint32_t rank0 = blockIdx.z * 16u * RT;
-    const bool inside = col < len;
-    const E* rows = static_cast<const E*>(a.rows[which].p) + (inside ? col : 0u);
-    const uint64_t stride = a.rows[which].stride;
-    const E* pieces = static_cast<const E*>(a.pieces[which]);
-
-    f32x4 acc[RT][VEC] = {};
-    for (uint32_t t0 = wave * STEP; t0 < (uint32_t)chunk.count; t0 += 4u * STEP) {
-        u32x4 in[VEC], turned[VEC];
+    constexpr uint32_t VEC = X::VEC;
+    const uint32_t lane = threadIdx.x & 63u, lo = lane & 15u, g = lane >> 4;
+    const E* pieces = static_cast<const E*>(a.pieces) + ((uint64_t)tile * a.rp + rank0 + lo) * X::PIECES * 64u + t0 % kTile + VEC * g;
+    V wf[RT][X::PIECES];
 #pragma unroll
-        for (uint32_t i = 0; i < VEC; ++i) {
-            const uint32_t t = t0 + VEC * g + i;
-            in[i] = u32x4{0u, 0u, 0u, 0u};  // tokens behind the chunk: zeros on both sides
-            if (t < (uint32_t)chunk.count) in[i] = load16<u32x4>(rows + (uint64_t)order[t] * stride);
-        }
-        const uint32_t tile = (uint32_t)chunk.tile + t0 / kTile;
-        V wf[RT][X::PIECES];
+    for (int j = 0; j < RT; ++j)
+#pragma unroll
+        for (uint32_t p = 0; p < X::PIECES; ++p) wf[j][p] = load16<V>(pieces + (16u * j * X::PIECES + p) * 64u);
+    u32x4 turned[VEC];
+    turn_over(in, turned);
+    if constexpr (X::SCALED) {
+        const float down = a.down[tile];
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+            for (uint32_t c = 0; c < VEC; ++c) {
+                f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (uint32_t p = 0; p < X::PIECES; ++p) d = X::mma(wf[j][p], __builtin_bit_cast(V, turned[c]), d);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[j][c][q] = __builtin_fmaf(d[q], down, acc[j][c][q]);
+            }
+    } else {
 #pragma unroll
         for (int j = 0; j < RT; ++j)
 #pragma unroll
             for (uint32_t p = 0; p < X::PIECES; ++p)
-                wf[j][p] = load16<V>(pieces + (((uint64_t)tile * a.rp + rank0 + 16u * j + lo) * X::PIECES + p) * 64u + t0 % kTile + VEC * g);
-        turn_over(in, turned);
-        if constexpr (X::SCALED) {
-            const float down = a.down[which][tile];
 #pragma unroll
-            for (int j = 0; j < RT; ++j)
-#pragma unroll
-                for (uint32_t c = 0; c < VEC; ++c) {
-                    f32x4 d = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (uint32_t p = 0; p < X::PIECES; ++p) d = X::mma(wf[j][p], __builtin_bit_cast(V, turned[c]), d);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) acc[j][c][q] = __builtin_fmaf(d[q], down, acc[j][c][q]);
-                }
-        } else {
-#pragma unroll
-            for (int j = 0; j < RT; ++j)
-#pragma unroll
-                for (uint32_t p = 0; p < X::PIECES; ++p)
-#pragma unroll
-                    for (uint32_t c = 0; c < VEC; ++c) acc[j][c] = X::mma(wf[j][p], __builtin_bit_cast(V, turned[c]), acc[j][c]);
-        }
+                for (uint32_t c = 0; c < VEC; ++c) acc[j][c] = X::mma(wf[j][p], __builtin_bit_cast(V, turned[c]), acc[j][c]);
     }
-#pragma unroll
-    for (uint32_t half = 2; half; half >>= 1) {
-        if (wave >= half && wave < 2u * half) {
-#pragma unroll
-            for (int j = 0; j < RT; ++j)
-#pragma unroll
-                for (uint32_t c = 0; c < VEC; ++c) red[(((wave - half) * RT + j) * VEC + c) * 64u + lane] = acc[j][c];
-        }
-        __syncthreads();
-        if (wave < half) {
-#pragma unroll
-            for (int j = 0; j < RT; ++j)
-#pragma unroll
-                for (uint32_t c = 0; c < VEC; ++c) acc[j][c] += red[((wave * RT + j) * VEC + c) * 64u + lane];
-        }
-        __syncthreads();
-    }
-    if (wave || !inside) return;
-    // lane: columns col ... col + VEC - 1, ranks rank0 + 16 j + 4 g + q
-    const uint64_t per = (uint64_t)a.rank * (a.len[0] + a.len[1]);
-    float* part = chunk.slot >= 0 ? a.partials + (uint64_t)chunk.slot * per + (which ? (uint64_t)a.rank * a.len[0] : 0u) : nullptr;
-    E* grad = static_cast<E*>(a.grad[which]) + (uint64_t)chunk.adapter * a.rank * len;
+}
+
+// A wavefront's sums: columns col ... col + VEC - 1, ranks rank0 + 16 j + 4 g + q.  To the chunk's partial sums, or
+// rounded to the gradient where the adapter has no other chunk.
+template <class E, int RT, bool DB>
+__device__ __forceinline__ void store_weights(const WeightArgs& a, const Chunk& chunk, uint32_t rank0, uint32_t col, const f32x4 (&acc)[RT][Mx<E>::VEC])
+{
+    using V = typename Mx<E>::V;
+    typedef E E4 __attribute__((ext_vector_type(4)));
+    constexpr uint32_t VEC = Mx<E>::VEC;
+    const uint32_t g = (threadIdx.x & 63u) >> 4, len = DB ? a.N : a.K;
+    if (col >= len) return;
+    const uint64_t per = (uint64_t)a.rank * (a.K + (uint64_t)a.N);
+    float* part = chunk.slot >= 0 ? a.partials + (uint64_t)chunk.slot * per + (DB ? (uint64_t)a.rank * a.K : 0u) : nullptr;
+    E* grad = static_cast<E*>(a.grad) + (uint64_t)chunk.adapter * a.rank * len;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
         const uint32_t r = rank0 + 16u * j + 4u * g;
         if (r >= a.rank) continue;
-        if (which) {  // [n][rank]
+        if (DB) {  // [n][rank]
 #pragma unroll
             for (uint32_t c = 0; c < VEC; ++c) {
                 const uint64_t at = (uint64_t)(col + c) * a.rank + r;
                 if (part) {
                     *reinterpret_cast<f32x4*>(part + at) = acc[j][c];
                 } else {
-                    typedef E E4 __attribute__((ext_vector_type(4)));
                     E4 o;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) o[q] = (E)acc[j][c][q];
@@ -852,6 +813,157 @@ __global__ void __launch_bounds__(256) weight_rows_kernel(WeightArgs a)
     }
 }
 
+// dA.  Workgroup: a chunk of tokens of one adapter, 16 VEC columns of x, up to RT * 16 ranks.  A wavefront takes
+// every fourth step of STEP tokens; a lane reads 16 bytes of VEC consecutive tokens (the 16 lanes of a group
+// read 256 contiguous bytes of a row) and turns them over in registers, one byte permute for two values,
+// so the contraction over tokens needs no LDS.  The wavefronts' sums meet in LDS at the end.
+template <class E, int RT>
+__global__ void __launch_bounds__(256) weight_rows_kernel(WeightArgs a)
+{
+    using X = Mx<E>;
+    constexpr uint32_t VEC = X::VEC, STEP = X::STEP;
+    __shared__ f32x4 red[2 * RT * VEC * 64];
+    __shared__ int32_t order[kMaxChunk];
+    const PlanLayout L(a.tokens, a.n);
+    const Chunk chunk = reinterpret_cast<const Chunk*>(a.plan + L.chunks)[blockIdx.y];
+    if (blockIdx.y >= (uint32_t)a.plan[L.counts + 1u]) return;
+    const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), lo = lane & 15u, g = lane >> 4, count = (uint32_t)chunk.count;
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) order[i] = a.plan[L.order + (uint32_t)chunk.first + i];
+    __syncthreads();
+    const uint32_t col = blockIdx.x * 16u * VEC + VEC * lo, rank0 = blockIdx.z * 16u * RT;
+    const E* rows = static_cast<const E*>(a.rows.p) + (col < a.K ? col : 0u);
+
+    f32x4 acc[RT][VEC] = {};
+    for (uint32_t t0 = wave * STEP; t0 < count; t0 += 4u * STEP) {
+        u32x4 in[VEC];
+#pragma unroll
+        for (uint32_t i = 0; i < VEC; ++i) {
+            const uint32_t t = t0 + VEC * g + i;
+            in[i] = u32x4{0u, 0u, 0u, 0u};  // tokens behind the chunk: zeros on both sides
+            if (t < count) in[i] = load16<u32x4>(rows + (uint64_t)(uint32_t)order[t] * a.rows.stride);
+        }
+        weight_step<E, RT>(a, (uint32_t)chunk.tile + t0 / kTile, t0, rank0, in, acc);
+    }
+#pragma unroll
+    for (uint32_t half = 2; half; half >>= 1) {
+        if (wave >= half && wave < 2u * half) {
+#pragma unroll
+            for (int j = 0; j < RT; ++j)
+#pragma unroll
+                for (uint32_t c = 0; c < VEC; ++c) red[(((wave - half) * RT + j) * VEC + c) * 64u + lane] = acc[j][c];
+        }
+        __syncthreads();
+        if (wave < half) {
+#pragma unroll
+            for (int j = 0; j < RT; ++j)
+#pragma unroll
+                for (uint32_t c = 0; c < VEC; ++c) acc[j][c] += red[((wave * RT + j) * VEC + c) * 64u + lane];
+        }
+        __syncthreads();
+    }
+    if (wave == 0) store_weights<E, RT, false>(a, chunk, rank0, col, acc);
+}
+
+// dB and the parts of d, from one pass over dy, which is most of what the backward pass has to read.
+// Workgroup: a chunk of tokens of one adapter, a slice of 64 VEC columns of dy, up to RT * 16 ranks; a wavefront has
+// 16 VEC of the columns and all tokens, STEP at a time with the next requested.  For dB the lanes' registers
+// are turned over as above; for d the same registers go through LDS to become operands along the columns, B
+// stays in registers, and the four wavefronts' sums of a step meet in LDS (two buffers, one barrier a step).
+template <class E, int RT>
+__global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) gradient_rows_kernel(WeightArgs a)
+{
+    using X = Mx<E>;
+    using V = typename X::V;
+    using C = Contraction<E, RT, false>;
+    constexpr uint32_t VEC = X::VEC, STEP = X::STEP, SUBS = STEP / 16u, UNITS = SUBS * RT * 64u;
+    __shared__ __attribute__((aligned(16))) unsigned char own[4][STEP * 256u];
+    __shared__ f32x4 red[2][4][UNITS];
+    __shared__ int32_t order[kMaxChunk];
+    const PlanLayout L(a.tokens, a.n);
+    const Chunk chunk = reinterpret_cast<const Chunk*>(a.plan + L.chunks)[blockIdx.y];
+    if (blockIdx.y >= (uint32_t)a.plan[L.counts + 1u]) return;
+    const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), lo = lane & 15u, g = lane >> 4, count = (uint32_t)chunk.count;
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) order[i] = a.plan[L.order + (uint32_t)chunk.first + i];
+    __syncthreads();
+    const uint32_t base = (blockIdx.x * 4u + wave) * 16u * VEC, col = base + VEC * lo, rank0 = blockIdx.z * 16u * RT;
+    const bool inside = col < a.N;
+    const E* rows = static_cast<const E*>(a.rows.p) + (inside ? col : 0u);
+
+    // B of the wavefront's columns: operand j, step h, rank 16 j + lo, columns base + STEP h + VEC g ...
+    V bf[4][RT];
+#pragma unroll
+    for (uint32_t h = 0; h < 4; ++h)
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+            for (uint32_t e = 0; e < VEC; ++e) {
+                const uint32_t n = base + STEP * h + VEC * g + e, r = rank0 + 16u * j + lo;
+                const bool in = n < a.N && r < a.rank;
+                const E v = static_cast<const E*>(a.B)[((uint64_t)chunk.adapter * a.N + (in ? n : 0u)) * a.rank + (in ? r : 0u)];
+                bf[h][j][e] = in ? v : (E)0.0f;
+            }
+    f32x4 acc[RT][VEC] = {};
+    auto request = [&](u32x4 (&in)[VEC], uint32_t t0) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t i = 0; i < VEC; ++i) {
+            const uint32_t t = t0 + VEC * g + i;
+            in[i] = load16<u32x4>(rows + (uint64_t)(uint32_t)order[t < count ? t : count - 1u] * a.rows.stride);
+        }
+    };
+    auto work = [&](u32x4 (&in)[VEC], uint32_t t0, uint32_t buffer) __attribute__((always_inline)) {
+        const u32x4 zero = {0u, 0u, 0u, 0u};
+        unsigned char* const mine = own[wave];
+#pragma unroll
+        for (uint32_t i = 0; i < VEC; ++i) {
+            const uint32_t row = VEC * g + i;
+            in[i] = inside && t0 + row < count ? in[i] : zero;  // zeros on both sides of the sums
+            *reinterpret_cast<u32x4*>(mine + C::at(row, lo)) = in[i];
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (uint32_t s = 0; s < SUBS; ++s) {
+            f32x4 d[RT] = {};
+#pragma unroll
+            for (uint32_t h = 0; h < 4; ++h) {
+                const V x = *reinterpret_cast<const V*>(mine + C::at(16u * s + lo, 4u * h + g));
+#pragma unroll
+                for (int j = 0; j < RT; ++j) d[j] = X::mma(bf[h][j], x, d[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < RT; ++j) red[buffer][wave][(s * RT + j) * 64u + lane] = d[j];
+        }
+        weight_step<E, RT>(a, (uint32_t)chunk.tile + t0 / kTile, t0, rank0, in, acc);
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < (UNITS + kThreads - 1u) / kThreads; ++k) {
+            const uint32_t u = threadIdx.x + k * kThreads, l = u & 63u, j = u / 64u % RT, s = u / (64u * RT);
+            const uint32_t t = t0 + 16u * s + (l & 15u), r = 16u * j + 4u * (l >> 4);
+            if (u < UNITS && t < count) {
+                const f32x4 sum = (red[buffer][0][u] + red[buffer][1][u]) + (red[buffer][2][u] + red[buffer][3][u]);
+                float* P = a.P + ((uint64_t)blockIdx.x * a.tokens + (uint32_t)chunk.first + t) * a.rp + rank0 + r;
+                *reinterpret_cast<f32x4*>(P) = rank0 + r < a.rank ? sum : f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+    };
+    u32x4 p[VEC], q[VEC];
+    request(p, 0);
+    uint32_t t0 = 0;
+    for (; t0 + 2u * STEP < count; t0 += 2u * STEP) {
+        request(q, t0 + STEP);
+        work(p, t0, 0);
+        request(p, t0 + 2u * STEP);
+        work(q, t0 + STEP, 1);
+    }
+    if (t0 + STEP < count) {
+        request(q, t0 + STEP);
+        work(p, t0, 0);
+        work(q, t0 + STEP, 1);
+    } else {
+        work(p, t0, 0);
+    }
+    store_weights<E, RT, true>(a, chunk, rank0, col, acc);
+}
+
 struct WeightSumArgs {
     const int32_t* plan;
     const float* partials;
@@ -868,12 +980,13 @@ __global__ void __launch_bounds__(256) weight_sum_kernel(WeightSumArgs a)
     const PlanLayout L(a.tokens, a.n);
     const uint32_t ad = blockIdx.y;
     const uint32_t count = (uint32_t)(a.plan[L.starts + ad + 1u] - a.plan[L.starts + ad]);
-    if (count > 0u && count <= kChunk) return;  // complete already
-    const uint32_t chunks = (count + kChunk - 1u) / kChunk;
+    if (count > 0u && count <= L.chunk) return;  // complete already
+    const uint32_t chunks = (count + L.chunk - 1u) / L.chunk;
     const uint64_t first = (uint64_t)a.rank * a.len[0], per = first + (uint64_t)a.rank * a.len[1];
     const float* part = a.partials + (uint64_t)(uint32_t)a.plan[L.slot_start + ad] * per;
     for (uint64_t i = 4u * ((uint64_t)blockIdx.x * kThreads + threadIdx.x); i < per; i += 4u * (uint64_t)gridDim.x * kThreads) {
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
         for (uint32_t c = 0; c < chunks; ++c) sum += load16<f32x4>(part + c * per + i);
         E4 o;
 #pragma unroll
@@ -903,7 +1016,7 @@ uint32_t cut(uint64_t tiles, uint32_t blocks, uint32_t least, uint32_t most)
 #define MC 1024u
 #endif
 #ifndef ME
-#define ME 2048u
+#define ME 8192u
 #endif
 template <class F>
 void for_rank(uint32_t rp, F f)
@@ -976,19 +1089,21 @@ struct ForwardPlan {
 };
 
 struct BackwardPlan {
-    Cut c;  // contraction over N, expansion to K
-    Cut u;  // contraction over K as the forward pass does it, when its sums are not given
-    uint64_t P, at, bt, vectors, down, pieces[2], tile_down[2], partials, bytes;
+    Cut c;           // expansion to K; the contraction over N is by slices
+    Cut u;           // contraction over K as the forward pass does it, when its sums are not given
+    uint32_t slices; // of N
+    uint64_t P, at, vectors, down, pieces[2], tile_down[2], partials, bytes;
     explicit BackwardPlan(const mi_lora* d) : c(d, d->N, d->K), u(d, d->K, d->N)
     {
         const PlanLayout L(d->tokens, d->n_adapters);
         const uint64_t e = d->dtype == MI_F32 ? 4u : 2u;
         c.few = false;
         c.grid_tiles = c.max_tiles;
+        const uint32_t slice = 64u * elements_of(d->dtype);
+        c.splits = slices = (d->N + slice - 1u) / slice;
         Take take;
         P = take((c.sums() > u.sums() ? c.sums() : u.sums()) * d->tokens);  // in turn
         at = take((uint64_t)d->n_adapters * d->rank * d->K * e);
-        bt = take((uint64_t)d->n_adapters * d->rank * d->N * e);
         vectors = take(c.max_tiles * pieces_bytes(c.rp));
         down = take(c.max_tiles * 64u * 4u);
         for (int i = 0; i < 2; ++i) {
@@ -1070,36 +1185,50 @@ int backward(const mi_lora* d, const void* dy, const void* x, const void* A, con
                      d->tokens, d->n_adapters, d->rank, b.u.splits, shrunk != nullptr};
         if (!shrunk && (st = contract<E>(d, plan, rx, A, d->K, b.u, P, s)) != MI_OK) return st;
         if ((st = tile_vectors<E>(b.c, v, s)) != MI_OK) return st;
-        // d, both ways
-        const uint32_t across = (d->rank + 63u) / 64u;
-        TransposeArgs t{plan, {A, B}, {ws + b.at, ws + b.bt}, d->tokens, d->n_adapters, {d->rank, d->N}, {d->K, d->rank}, across * ((d->K + 63u) / 64u)};
-        hipLaunchKernelGGL((transpose_kernel<E>), dim3(t.blocks0 + across * ((d->N + 63u) / 64u), d->n_adapters), dim3(kThreads), 0, s, t);
-        if ((st = launch_status()) != MI_OK) return st;
-        if ((st = contract<E>(d, plan, rdy, ws + b.bt, d->N, b.c, P, s)) != MI_OK) return st;
+        const PlanLayout L(d->tokens, d->n_adapters);
+        const uint32_t rt = b.c.rp <= 64u ? b.c.rp : 64u, cols = 16u * Mx<E>::VEC;
+        auto for_weights = [&](auto f) {  // rank 128 as two halves
+            if (rt == 16u) f(std::integral_constant<int, 1>{});
+            else if (rt == 32u) f(std::integral_constant<int, 2>{});
+            else f(std::integral_constant<int, 4>{});
+            return launch_status();
+        };
+        // dB and d
+        float* partials = reinterpret_cast<float*>(ws + b.partials);
+        WeightArgs w{plan, rdy, ws + b.pieces[1], tile_down[1], partials, dB, B, P, d->tokens, d->n_adapters, d->rank, b.c.rp, d->K, d->N};
+        dim3 grid(b.slices, (uint32_t)L.max_chunks, b.c.rp / rt);
+        st = for_weights([&](auto r) {
+            hipLaunchKernelGGL((gradient_rows_kernel<E, decltype(r)::value>), grid, dim3(kThreads), 0, s, w);
+        });
+        if (st != MI_OK) return st;
         v.shrunk = nullptr;
         v.given = false;
-        v.splits = b.c.splits;
+        v.splits = b.slices;
         v.vectors = ws + b.vectors;
         v.down = down;
         v.pieces = ws + b.pieces[0];
         v.tile_down = tile_down[0];
         if ((st = tile_vectors<E>(b.c, v, s)) != MI_OK) return st;
+        // dx
+        TransposeArgs t{plan, A, ws + b.at, d->tokens, d->n_adapters, d->rank, d->K};
+        hipLaunchKernelGGL((transpose_kernel<E>), dim3((d->K + kThreads - 1u) / kThreads, d->rank / 8u, d->n_adapters), dim3(kThreads), 0, s, t);
+        if ((st = launch_status()) != MI_OK) return st;
         if ((st = expand<E>(b.c, {plan, {dx_in, d->out_stride}, dx, d->out_stride, ws + b.at, ws + b.vectors, down, nullptr, nullptr, nullptr,
                                   d->tokens, d->n_adapters, d->rank, d->K, 0, 0}, s)) != MI_OK)
             return st;
-        const PlanLayout L(d->tokens, d->n_adapters);
-        const uint32_t cols = 16u * Mx<E>::VEC, blocks0 = (d->K + cols - 1u) / cols, blocks1 = (d->N + cols - 1u) / cols;
-        WeightArgs w{plan, {rx, rdy}, {ws + b.pieces[0], ws + b.pieces[1]}, {tile_down[0], tile_down[1]}, reinterpret_cast<float*>(ws + b.partials),
-                     {dA, dB}, d->tokens, d->n_adapters, d->rank, b.c.rp, {d->K, d->N}, blocks0};
-        const uint32_t rt = b.c.rp <= 64u ? b.c.rp : 64u;
-        const dim3 grid(blocks0 + blocks1, (uint32_t)L.max_chunks, b.c.rp / rt);
-        if (rt == 16u) hipLaunchKernelGGL((weight_rows_kernel<E, 1>), grid, dim3(kThreads), 0, s, w);
-        else if (rt == 32u) hipLaunchKernelGGL((weight_rows_kernel<E, 2>), grid, dim3(kThreads), 0, s, w);
-        else hipLaunchKernelGGL((weight_rows_kernel<E, 4>), grid, dim3(kThreads), 0, s, w);
-        if ((st = launch_status()) != MI_OK) return st;
+        // dA
+        w.rows = rx;
+        w.pieces = ws + b.pieces[0];
+        w.down = tile_down[0];
+        w.grad = dA;
+        grid.x = (d->K + cols - 1u) / cols;
+        st = for_weights([&](auto r) {
+            hipLaunchKernelGGL((weight_rows_kernel<E, decltype(r)::value>), grid, dim3(kThreads), 0, s, w);
+        });
+        if (st != MI_OK) return st;
     }
     WeightSumArgs sum{plan, reinterpret_cast<float*>(ws + b.partials), {dA, dB}, d->tokens, d->n_adapters, d->rank, {d->K, d->N}};
-    hipLaunchKernelGGL((weight_sum_kernel<E>), dim3(64, d->n_adapters), dim3(kThreads), 0, s, sum);
+    hipLaunchKernelGGL((weight_sum_kernel<E>), dim3(512, d->n_adapters), dim3(kThreads), 0, s, sum);
     return launch_status();
 }
 

@@ -114,9 +114,10 @@ def test_plan_groups_tokens_in_order(pkg, T, n, bits):
     counts = torch.bincount(key, minlength=n + 1)
     starts = torch.cumsum(counts, 0) - counts
     assert torch.equal(plan.order.cpu().long(), order) and torch.equal(plan.starts.cpu().long(), starts)
-    # the tables of work: tiles of 64 and chunks of 512 tokens of one adapter
+    # the tables of work: tiles of 64 and chunks of 128 or 512 tokens of one adapter
     groups = min(T, n + 1)
-    max_tiles, max_chunks = T // 64 + groups, T // 512 + groups
+    size = 128 if T < 4096 else 512  # of a chunk
+    max_tiles, max_chunks = T // 64 + groups, T // size + groups
     buf = plan.buffer.cpu()
     n_tiles, n_chunks = buf[4 * max_tiles + 8 * max_chunks:][:2].tolist()
     tiles, chunks, slots, tile_of = [], [], 0, {}
@@ -126,12 +127,12 @@ def test_plan_groups_tokens_in_order(pkg, T, n, bits):
         tiles += [(a, first + i, min(64, left - i)) for i in range(0, left, 64)]
         if a == n:
             break
-        many = left > 512
-        for i in range(0, left, 512):
-            chunks.append((a, first + i, min(512, left - i), slots if many else -1, tile_of[a] + i // 64))
+        many = left > size
+        for i in range(0, left, size):
+            chunks.append((a, first + i, min(size, left - i), slots if many else -1, tile_of[a] + i // 64))
             slots += many
     assert (n_tiles, n_chunks) == (len(tiles), len(chunks)) and n_tiles <= max_tiles and n_chunks <= max_chunks
-    assert slots <= 2 * (T // 512)
+    assert slots <= 2 * (T // size)
     assert buf[:4 * n_tiles].view(-1, 4)[:, :3].tolist() == [list(t) for t in tiles]
     assert buf[4 * max_tiles:][:8 * n_chunks].view(-1, 8)[:, :5].tolist() == [list(c) for c in chunks]
 
