@@ -30,7 +30,7 @@ struct PlanLayout {
     {
         const uint64_t groups = tokens < n + 1ull ? tokens : n + 1ull;  // at most so many are not empty
         max_tiles = tokens / kTile + groups;
-        chunk = tokens < 4096u ? 128u : 512u;
+        chunk = tokens < 4096u ? 128u : tokens < 8192u ? 256u : 512u;
         max_chunks = tokens / chunk + groups;
         // only adapters with more than `chunk` tokens have slots: at most tokens / chunk of them, and
         // ceil(c / chunk) <= 2 c / chunk for each

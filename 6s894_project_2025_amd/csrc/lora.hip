@@ -813,7 +813,9 @@ __device__ __forceinline__ void store_weights(const WeightArgs& a, const Chunk& 
     }
 }
 
-// dA.  Workgroup: a chunk of tokens of one adapter, 16 VEC columns of x, up to RT * 16 ranks.  A wavefront takes
+// dA.  Workgroup: a chunk of tokens of one adapter, 16 VEC columns of x, RT * 16 ranks (32 at most: with 64 the
+// registers leave one wavefront per SIMD: a backward pass of 8192 tokens, 4096 -> 4096, rank 64 took 130 us
+// against 109, though rows are then read once less).  A wavefront takes
 // every fourth step of STEP tokens; a lane reads 16 bytes of VEC consecutive tokens (the 16 lanes of a group
 // read 256 contiguous bytes of a row) and turns them over in registers, one byte permute for two values,
 // so the contraction over tokens needs no LDS.  The wavefronts' sums meet in LDS at the end.
@@ -870,7 +872,7 @@ __global__ void __launch_bounds__(256) weight_rows_kernel(WeightArgs a)
 // are turned over as above; for d the same registers go through LDS to become operands along the columns, B
 // stays in registers, and the four wavefronts' sums of a step meet in LDS (two buffers, one barrier a step).
 template <class E, int RT>
-__global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) gradient_rows_kernel(WeightArgs a)
+__global__ void __launch_bounds__(256, RT == 2 ? 1 : 2) gradient_rows_kernel(WeightArgs a)
 {
     using X = Mx<E>;
     using V = typename X::V;
@@ -885,7 +887,8 @@ __global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) gradient_rows_kernel(Wei
     const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), lo = lane & 15u, g = lane >> 4, count = (uint32_t)chunk.count;
     for (uint32_t i = threadIdx.x; i < count; i += kThreads) order[i] = a.plan[L.order + (uint32_t)chunk.first + i];
     __syncthreads();
-    const uint32_t base = (blockIdx.x * 4u + wave) * 16u * VEC, col = base + VEC * lo, rank0 = blockIdx.z * 16u * RT;
+    const uint32_t slice = blockIdx.x, rank0 = blockIdx.z * 16u * RT;
+    const uint32_t base = (slice * 4u + wave) * 16u * VEC, col = base + VEC * lo;
     const bool inside = col < a.N;
     const E* rows = static_cast<const E*>(a.rows.p) + (inside ? col : 0u);
 
@@ -940,7 +943,7 @@ __global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) gradient_rows_kernel(Wei
             const uint32_t t = t0 + 16u * s + (l & 15u), r = 16u * j + 4u * (l >> 4);
             if (u < UNITS && t < count) {
                 const f32x4 sum = (red[buffer][0][u] + red[buffer][1][u]) + (red[buffer][2][u] + red[buffer][3][u]);
-                float* P = a.P + ((uint64_t)blockIdx.x * a.tokens + (uint32_t)chunk.first + t) * a.rp + rank0 + r;
+                float* P = a.P + ((uint64_t)slice * a.tokens + (uint32_t)chunk.first + t) * a.rp + rank0 + r;
                 *reinterpret_cast<f32x4*>(P) = rank0 + r < a.rank ? sum : f32x4{0.f, 0.f, 0.f, 0.f};
             }
         }
@@ -1186,11 +1189,10 @@ int backward(const mi_lora* d, const void* dy, const void* x, const void* A, con
         if (!shrunk && (st = contract<E>(d, plan, rx, A, d->K, b.u, P, s)) != MI_OK) return st;
         if ((st = tile_vectors<E>(b.c, v, s)) != MI_OK) return st;
         const PlanLayout L(d->tokens, d->n_adapters);
-        const uint32_t rt = b.c.rp <= 64u ? b.c.rp : 64u, cols = 16u * Mx<E>::VEC;
-        auto for_weights = [&](auto f) {  // rank 128 as two halves
+        const uint32_t rt = b.c.rp <= 32u ? b.c.rp : 32u, cols = 16u * Mx<E>::VEC;
+        auto for_weights = [&](auto f) {
             if (rt == 16u) f(std::integral_constant<int, 1>{});
-            else if (rt == 32u) f(std::integral_constant<int, 2>{});
-            else f(std::integral_constant<int, 4>{});
+            else f(std::integral_constant<int, 2>{});
             return launch_status();
         };
         // dB and d

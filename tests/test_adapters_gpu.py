@@ -114,9 +114,9 @@ def test_plan_groups_tokens_in_order(pkg, T, n, bits):
     counts = torch.bincount(key, minlength=n + 1)
     starts = torch.cumsum(counts, 0) - counts
     assert torch.equal(plan.order.cpu().long(), order) and torch.equal(plan.starts.cpu().long(), starts)
-    # the tables of work: tiles of 64 and chunks of 128 or 512 tokens of one adapter
+    # the tables of work: tiles of 64 and chunks of 128 to 512 tokens of one adapter
     groups = min(T, n + 1)
-    size = 128 if T < 4096 else 512  # of a chunk
+    size = 128 if T < 4096 else 256 if T < 8192 else 512  # of a chunk
     max_tiles, max_chunks = T // 64 + groups, T // size + groups
     buf = plan.buffer.cpu()
     n_tiles, n_chunks = buf[4 * max_tiles + 8 * max_chunks:][:2].tolist()
