@@ -9,6 +9,7 @@ recorded; :func:`lora_add_backward` computes the gradients.
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 
 import torch
@@ -43,9 +44,21 @@ class AdapterPlan:
         return self.buffer[self._starts:self._starts + self.n_adapters + 1]
 
 
+@functools.lru_cache(maxsize=1024)
+def _layout(tokens: int, n_adapters: int) -> tuple[int, int, int]:
+    out = (ctypes.c_uint64 * 3)()
+    _lib.check(_lib.load().mi_adapter_plan_layout(tokens, n_adapters, out), "adapter_plan")
+    return tuple(out)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(sizes: bytes, backward: int) -> int:
+    return max(_lib.load().mi_lora_workspace(sizes, backward), 16)
+
+
 def adapter_plan(ids: torch.Tensor, n_adapters: int) -> AdapterPlan:
     """Groups a batch's tokens by adapter: ``ids`` (int32 or int64, ``[tokens]``, on the GPU) names each
-    token's adapter in ``[0, n_adapters)``; any other value means none.  One kernel and no
+    token's adapter in ``[0, n_adapters)``; any other value means none.  No
     synchronisation, so it can be captured with the rest of a step.  The plan serves every
     :func:`lora_add` and :func:`lora_add_backward` on this batch.
     """
@@ -58,9 +71,7 @@ def adapter_plan(ids: torch.Tensor, n_adapters: int) -> AdapterPlan:
         raise RuntimeError(f"at most {MAX_TOKENS} tokens, got {T}")
     _require_cuda(ids, "ids")
     lib = _lib.load()
-    layout = (ctypes.c_uint64 * 3)()
-    _lib.check(lib.mi_adapter_plan_layout(T, n_adapters, layout), "adapter_plan")
-    size, order, starts = layout
+    size, order, starts = _layout(T, n_adapters)
     ids = ids.contiguous()
     buffer = torch.empty(size, dtype=torch.int32, device=ids.device)
     with _on_device_of(ids):
@@ -74,6 +85,10 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.size(0) > 1 else 0
 
 
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _readable(t: torch.Tensor) -> torch.Tensor:
     """``t`` if its rows are contiguous and 16-byte aligned, else a dense copy."""
     if t.numel() == 0 or (t.stride(1) == 1 and t.data_ptr() % 16 == 0 and _row_stride(t) * t.element_size() % 16 == 0):
@@ -82,6 +97,24 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
 
 
 def _check(y, x, A, B, plan, scales, name):
+    """Sizes of a call; anything wrong goes to :func:`_refuse`, which says what."""
+    dt, dev = x.dtype, x.get_device()
+    try:
+        (T, K), (Ty, N), (n, r, KA), nNr = x.shape, y.shape, A.shape, B.shape
+    except ValueError:
+        _refuse(y, x, A, B, plan, scales, name)
+    if (dt in _DTYPE_CODE and y.dtype is dt and A.dtype is dt and B.dtype is dt
+            and Ty == T and KA == K and nNr == (n, N, r)
+            and r % 8 == 0 and 8 <= r <= MAX_RANK and K % 8 == 0 and N % 8 == 0 and 8 <= K <= MAX_WIDTH and 8 <= N <= MAX_WIDTH
+            and plan.tokens == T and plan.n_adapters == n
+            and dev >= 0 and y.get_device() == dev and A.get_device() == dev and B.get_device() == dev
+            and plan.buffer.get_device() == dev
+            and (scales is None or (scales.dtype is torch.float32 and scales.shape == (n,) and scales.get_device() == dev))):
+        return T, n, r, K, N
+    _refuse(y, x, A, B, plan, scales, name)
+
+
+def _refuse(y, x, A, B, plan, scales, name):
     for t, n, dims in ((y, name, 2), (x, "x", 2), (A, "A", 3), (B, "B", 3)):
         if t.dim() != dims:
             raise RuntimeError(f"{n} must have {dims} dimensions, got {tuple(t.shape)}")
@@ -103,7 +136,7 @@ def _check(y, x, A, B, plan, scales, name):
     for t, what in ((y, name), (A, "A"), (B, "B"), (plan.buffer, "plan"), (scales, "scales")):
         if t is not None and t.device != x.device:
             raise RuntimeError(f"{what} must be on x's device {x.device}, got {t.device}")
-    return T, n, r, K, N
+    raise RuntimeError(f"x must be on a GPU (got {x.device})")
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, plan: AdapterPlan,
@@ -124,17 +157,17 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     if inplace and ((T > 1 and y.stride(0) == 0) or y.stride(1) == 0):
         raise RuntimeError("inplace needs rows that do not share memory (an expanded y was given)")
     ys, xs, Ac, Bc = _readable(y), _readable(x), _dense16(A), _dense16(B)
-    out = ys if inplace else torch.empty((T, N), dtype=y.dtype, device=y.device)
+    out = ys if inplace else torch.empty_like(ys, memory_format=torch.contiguous_format)
     shrunk = torch.empty((T, r), dtype=torch.float32, device=x.device) if return_shrunk else None
     if T:
         sc = None if scales is None else scales.contiguous()
         sizes = _LORA.pack(T, _row_stride(xs), _row_stride(ys), _row_stride(out), n, r, K, N, _DTYPE_CODE[x.dtype])
         lib = _lib.load()
-        workspace = torch.empty(lib.mi_lora_workspace(sizes, 0), dtype=torch.uint8, device=x.device)
+        workspace = torch.empty(_workspace_bytes(sizes, 0), dtype=torch.uint8, device=x.device)
         with _on_device_of(x):
             st = lib.mi_lora_add(ys.data_ptr(), xs.data_ptr(), Ac.data_ptr(), Bc.data_ptr(),
-                                 None if sc is None else sc.data_ptr(), plan.buffer.data_ptr(), out.data_ptr(),
-                                 None if shrunk is None else shrunk.data_ptr(), workspace.data_ptr(), sizes, _stream(x))
+                                 _ptr(sc), plan.buffer.data_ptr(), out.data_ptr(),
+                                 _ptr(shrunk), workspace.data_ptr(), sizes, _stream(x))
         _lib.check(st, "lora_add")
     if inplace:
         if ys is not y:
@@ -163,18 +196,17 @@ def lora_add_backward(dy: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: tor
         if (T > 1 and dx.stride(0) == 0) or dx.stride(1) == 0:
             raise RuntimeError("dx needs rows that do not share memory (an expanded tensor was given)")
     gs, xs, Ac, Bc = _readable(dy), _readable(x), _dense16(A), _dense16(B)
-    into = torch.empty((T, K), dtype=x.dtype, device=dev) if dx is None else _readable(dx)
-    dA = torch.empty((n, r, K), dtype=A.dtype, device=dev)
-    dB = torch.empty((n, N, r), dtype=B.dtype, device=dev)
+    into = torch.empty_like(xs, memory_format=torch.contiguous_format) if dx is None else _readable(dx)
+    dA, dB = torch.empty_like(Ac), torch.empty_like(Bc)
     sc = None if scales is None else scales.contiguous()
     u = None if shrunk is None else shrunk.contiguous()
     sizes = _LORA.pack(T, _row_stride(xs), _row_stride(gs), _row_stride(into), n, r, K, N, _DTYPE_CODE[x.dtype])
     lib = _lib.load()
-    workspace = torch.empty(max(lib.mi_lora_workspace(sizes, 1), 16), dtype=torch.uint8, device=dev)
+    workspace = torch.empty(_workspace_bytes(sizes, 1), dtype=torch.uint8, device=dev)
     with _on_device_of(x):
         st = lib.mi_lora_add_backward(gs.data_ptr(), xs.data_ptr(), Ac.data_ptr(), Bc.data_ptr(),
-                                      None if sc is None else sc.data_ptr(), plan.buffer.data_ptr(),
-                                      None if u is None else u.data_ptr(), None if dx is None else into.data_ptr(),
+                                      _ptr(sc), plan.buffer.data_ptr(),
+                                      _ptr(u), None if dx is None else into.data_ptr(),
                                       into.data_ptr(), dA.data_ptr(), dB.data_ptr(), workspace.data_ptr(), sizes, _stream(x))
     _lib.check(st, "lora_add_backward")
     if dx is not None:

@@ -24,14 +24,15 @@ struct Chunk {  // slot: row of partial sums, or -1 where the adapter has no oth
 struct PlanLayout {
     uint32_t chunk;  // tokens of one adapter behind one partial weight gradient: few where there are few to share out
     uint64_t max_tiles, max_chunks, max_slots;
-    uint64_t chunks, counts, slot_start, order, starts, size;  // offsets in int32; tiles are at 0
+    uint64_t chunks, counts, slot_start, order, starts, histograms, size;  // offsets in int32; tiles are at 0
+    uint32_t groups;  // workgroups that sort, each with a histogram, where one is too few; 0: one does everything
 
     __host__ __device__ PlanLayout(uint64_t tokens, uint32_t n)
     {
-        const uint64_t groups = tokens < n + 1ull ? tokens : n + 1ull;  // at most so many are not empty
-        max_tiles = tokens / kTile + groups;
+        const uint64_t used = tokens < n + 1ull ? tokens : n + 1ull;  // at most so many adapters
+        max_tiles = tokens / kTile + used;
         chunk = tokens < 4096u ? 128u : tokens < 8192u ? 256u : 512u;
-        max_chunks = tokens / chunk + groups;
+        max_chunks = tokens / chunk + used;
         // only adapters with more than `chunk` tokens have slots: at most tokens / chunk of them, and
         // ceil(c / chunk) <= 2 c / chunk for each
         max_slots = 2u * (tokens / chunk);
@@ -40,7 +41,9 @@ struct PlanLayout {
         slot_start = counts + 2u;           // [n]
         order = slot_start + n;             // [tokens]
         starts = order + tokens;            // [n + 1]
-        size = starts + n + 1u;
+        histograms = starts + n + 1u;
+        groups = tokens <= 4096u ? 0u : tokens <= 256u * 1024u ? (uint32_t)((tokens + 1023u) / 1024u) : 256u;
+        size = histograms + (uint64_t)groups * (n + 1u);
     }
 };
 

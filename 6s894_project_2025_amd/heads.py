@@ -19,24 +19,56 @@ _HEADS = struct.Struct("<Q6Q6Q4I" "I4I" "iiIII" "f4x")  # mi_heads
 _MAX_D = 512
 
 
-def _head_strides(t: torch.Tensor) -> tuple[int, int]:
-    """Token and head stride in elements; 0 along an axis of one entry, whose stride means nothing."""
-    return (t.stride(0) if t.size(0) > 1 else 0, t.stride(1) if t.size(1) > 1 else 0)
+def _readable(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """``t`` as the kernels address it (heads contiguous, 16-byte aligned base and strides), a dense copy if it is
+    not, with its token and head stride in elements; 0 along an axis of one entry, whose stride means nothing."""
+    T, H, D = t.shape
+    ts, hs, ds = t.stride()
+    if T <= 1:
+        ts = 0
+    if H <= 1:
+        hs = 0
+    align = 15 // t.element_size()  # a power of two less one
+    if ds == 1 and not (ts | hs) & align and t.data_ptr() % 16 == 0 or T * H == 0:
+        return t, ts, hs
+    return t.clone(memory_format=torch.contiguous_format), H * D, D
 
 
-def _laid_out(t: torch.Tensor) -> bool:
-    """Heads contiguous, 16-byte aligned base and strides: what the kernels address directly."""
-    e = t.element_size()
-    return (t.numel() == 0 or
-            (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in _head_strides(t))))
+def _describe(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, interleaved, hadamard):
+    """The operands that both directions share: (tokens, heads, D and the rest of mi_heads behind the strides).
+    Anything wrong goes to :func:`_refuse`, which says what."""
+    dt, dev = q.dtype, q.get_device()
+    try:
+        (T, Hq, D), (Tk, Hk, Dk), (half,), pshape = q.shape, k.shape, inv_freq.shape, positions.shape
+    except ValueError:
+        _refuse(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, hadamard)
+    axes = 1 if len(pshape) == 1 else pshape[0] if len(pshape) == 2 else 0
+    if sections is None:
+        ends = (half, 0, 0, 0)
+        fits = axes == 1
+    else:
+        ends, total = [], 0
+        for s in sections:
+            total += int(s)
+            ends.append(total)
+        fits = 1 <= len(ends) == axes <= 4 and total == half and min(sections) >= 0
+        ends += [0] * (4 - axes)
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    wdt = weights[0].dtype if weights else dt
+    if not (fits and dt in _DTYPE_CODE and k.dtype is dt and Tk == T and Dk == D and D % 16 == 0 and 16 <= D <= _MAX_D
+            and eps >= 0.0 and half % 8 == 0 and 2 * half <= D and pshape[-1] == T
+            and (positions.dtype is torch.int32 or positions.dtype is torch.int64)
+            and (inv_freq.dtype is torch.float32 or inv_freq.dtype is torch.float64)
+            and (wdt is dt or wdt is torch.float32) and not (hadamard and not _is_pow2(D))
+            and all(w.shape == (D,) and w.dtype is wdt and w.get_device() == dev for w in weights)
+            and dev >= 0 and k.get_device() == dev and positions.get_device() == dev and inv_freq.get_device() == dev):
+        _refuse(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, hadamard)
+    flags = (_NEIGHBOURS if interleaved else 0) | (_HADAMARD if hadamard else 0)
+    return T, D, wdt, (Hq, Hk, D, 2 * half, axes, *ends, _DTYPE_CODE[dt], _DTYPE_CODE[wdt], 8 * positions.element_size(),
+                       8 * inv_freq.element_size(), flags, eps)
 
 
-def _readable(t: torch.Tensor) -> torch.Tensor:
-    return t if _laid_out(t) else t.clone(memory_format=torch.contiguous_format)
-
-
-def _describe(name, q, k, q_weight, k_weight, positions, inv_freq, eps, sections, interleaved, hadamard):
-    """Checks the operands that both directions share; returns (D, R, flags, axes, section ends)."""
+def _refuse(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, hadamard):
     for t, n in ((q, "q"), (k, "k")):
         if t.dim() != 3:
             raise RuntimeError(f"{n} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
@@ -65,7 +97,6 @@ def _describe(name, q, k, q_weight, k_weight, positions, inv_freq, eps, sections
     if sections is None:
         if axes != 1:
             raise RuntimeError("positions with several axes need sections")
-        ends = [half]
     else:
         ends, total = [], 0
         for s in sections:
@@ -75,7 +106,6 @@ def _describe(name, q, k, q_weight, k_weight, positions, inv_freq, eps, sections
             ends.append(total)
         if len(ends) != axes or total != half:
             raise RuntimeError(f"sections {tuple(sections)} must give each of the {axes} axes its share of the {half} frequencies")
-    ends += [0] * (4 - axes)
     kinds = set()
     for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is None:
@@ -87,23 +117,12 @@ def _describe(name, q, k, q_weight, k_weight, positions, inv_freq, eps, sections
         kinds.add(w.dtype)
     if len(kinds) > 1:
         raise RuntimeError("q_weight and k_weight must share a dtype")
-    weight_dtype = kinds.pop() if kinds else q.dtype
     _require_cuda(q, "q")
     for t, n in ((k, "k"), (q_weight, "q_weight"), (k_weight, "k_weight"), (positions, "positions"),
                  (inv_freq, "inv_freq")):
         if t is not None and t.device != q.device:
             raise RuntimeError(f"{n} must be on q's device {q.device}, got {t.device}")
-    flags = (_NEIGHBOURS if interleaved else 0) | (_HADAMARD if hadamard else 0)
-    return D, 2 * half, flags, axes, ends, weight_dtype
-
-
-def _pack(q, k, tensors, D, R, flags, axes, ends, weight_dtype, positions, inv_freq, eps) -> bytes:
-    token, head = [0] * 6, [0] * 6
-    for i, t in enumerate(tensors):
-        token[i], head[i] = _head_strides(t)
-    return _HEADS.pack(q.size(0), *token, *head, q.size(1), k.size(1), D, R, axes, *ends,
-                       _DTYPE_CODE[q.dtype], _DTYPE_CODE[weight_dtype], 8 * positions.element_size(),
-                       8 * inv_freq.element_size(), flags, eps)
+    raise RuntimeError("unsupported operands")
 
 
 def _ptr(t):
@@ -127,27 +146,25 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     positions keep their accuracy; the rest is fp32 with one rounding at the end.
     ``inplace=True`` writes into ``q`` and ``k`` and returns them.
     """
-    D, R, flags, axes, ends, wdt = _describe("qk_norm_rope", q, k, q_weight, k_weight, positions, inv_freq, eps,
-                                             sections, interleaved, hadamard)
+    T, D, _, rest = _describe(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, interleaved, hadamard)
     _no_graph("qk_norm_rope", q, k, q_weight, k_weight)
     if inplace and any(n > 1 and s == 0 for t in (q, k) for n, s in zip(t.shape, t.stride())):
         raise RuntimeError("inplace needs heads that do not share memory (an expanded tensor was given)")
-    qs, ks = _readable(q), _readable(k)
+    (qs, qt, qh), (ks, kt, kh) = _readable(q), _readable(k)
     if inplace:
-        qo, ko = qs, ks
+        qo, ko, qot, qoh, kot, koh = qs, ks, qt, qh, kt, kh
     else:
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    if q.numel() or k.numel():
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+        qot, qoh, kot, koh = rest[0] * D, D, rest[1] * D, D
+    if qo.numel() or ko.numel():
         qw = None if q_weight is None else _dense16(q_weight)
         kw = None if k_weight is None else _dense16(k_weight)
         pos, freq = positions.contiguous(), inv_freq.contiguous()
         lib = _lib.load()
         with _on_device_of(q):
-            st = lib.mi_qk_norm_rope(qs.data_ptr(), ks.data_ptr(), _ptr(qw), _ptr(kw), pos.data_ptr(), freq.data_ptr(),
-                                     qo.data_ptr(), ko.data_ptr(),
-                                     _pack(qs, ks, (qs, ks, qo, ko), D, R, flags, axes, ends, wdt, pos, freq, eps),
-                                     _stream(q))
+            st = lib.mi_qk_norm_rope(qs.data_ptr(), ks.data_ptr(), _ptr(qw), _ptr(kw), pos.data_ptr(), freq.data_ptr(), qo.data_ptr(),
+                                     ko.data_ptr(), _HEADS.pack(T, qt, kt, qot, kot, 0, 0, qh, kh, qoh, koh, 0, 0, *rest), _stream(q))
         _lib.check(st, "qk_norm_rope")
     if inplace:
         if qs is not q:
@@ -167,32 +184,31 @@ def qk_norm_rope_backward(q_grad: torch.Tensor, k_grad: torch.Tensor, q: torch.T
     ``None`` has gradient ``None``; the others are in the weights' dtype, summed over all tokens and
     heads in fp32 in a fixed order.
     """
-    D, R, flags, axes, ends, wdt = _describe("qk_norm_rope_backward", q, k, q_weight, k_weight, positions, inv_freq,
-                                             eps, sections, interleaved, hadamard)
+    T, D, wdt, rest = _describe(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, interleaved, hadamard)
     for g, t, n in ((q_grad, q, "q_grad"), (k_grad, k, "k_grad")):
-        if g.shape != t.shape or g.dtype != t.dtype:
+        if g.shape != t.shape or g.dtype is not t.dtype:
             raise RuntimeError(f"{n} must have the shape and dtype of {n[0]}: {tuple(t.shape)} {t.dtype}, got "
                                f"{tuple(g.shape)} {g.dtype}")
-        if g.device != q.device:
+        if g.device != t.device:
             raise RuntimeError(f"{n} must be on q's device {q.device}, got {g.device}")
     dev = q.device
-    dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dk = torch.empty_like(k, memory_format=torch.contiguous_format)
     dqw = None if q_weight is None else torch.empty(D, dtype=wdt, device=dev)
     dkw = None if k_weight is None else torch.empty(D, dtype=wdt, device=dev)
-    qs, ks, qg, kg = _readable(q), _readable(k), _readable(q_grad), _readable(k_grad)
+    (qs, qt, qh), (ks, kt, kh), (qg, qgt, qgh), (kg, kgt, kgh) = _readable(q), _readable(k), _readable(q_grad), _readable(k_grad)
     qw = None if q_weight is None else _dense16(q_weight)
     kw = None if k_weight is None else _dense16(k_weight)
     pos, freq = positions.contiguous(), inv_freq.contiguous()
     lib = _lib.load()
     workspace = None
     if dqw is not None or dkw is not None:
-        workspace = torch.empty(lib.mi_qk_norm_rope_workspace(q.size(0), D), dtype=torch.uint8, device=dev)
+        workspace = torch.empty(lib.mi_qk_norm_rope_workspace(T, D), dtype=torch.uint8, device=dev)
     with _on_device_of(q):
         st = lib.mi_qk_norm_rope_backward(qs.data_ptr(), ks.data_ptr(), qg.data_ptr(), kg.data_ptr(), _ptr(qw), _ptr(kw),
                                           pos.data_ptr(), freq.data_ptr(), dq.data_ptr(), dk.data_ptr(), _ptr(dqw), _ptr(dkw),
                                           _ptr(workspace),
-                                          _pack(qs, ks, (qs, ks, qg, kg, dq, dk), D, R, flags, axes, ends, wdt, pos, freq, eps),
+                                          _HEADS.pack(T, qt, kt, qgt, kgt, rest[0] * D, rest[1] * D, qh, kh, qgh, kgh, D, D, *rest),
                                           _stream(q))
     _lib.check(st, "qk_norm_rope_backward")
     return dq, dk, dqw, dkw

@@ -143,7 +143,7 @@ int mi_fp8_gemm_rowscale(const void* qa, const float* sa, const void* qb, const 
  *                                          one in their own order, those without an adapter last)
  *   plan[layout[2] + a], a <= n_adapters : first position of adapter a; [n_adapters] of the tokens without
  * The rest is the kernels' own.  tokens <= 2^24, 1 <= n_adapters <= 1024, id_bits 32 or 64.
- * One kernel; the result depends on the ids alone.  No counterpart in the reference.
+ * One kernel up to 4096 tokens, two beyond; the result depends on the ids alone.  No counterpart in the reference.
  */
 int mi_adapter_plan(const void* ids, int id_bits, uint64_t tokens, uint32_t n_adapters, int32_t* plan,
                     void* stream);

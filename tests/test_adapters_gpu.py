@@ -100,7 +100,8 @@ def on_gpu(c):
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 64])
 @pytest.mark.parametrize("T,n", [(0, 3), (1, 1), (1, 1024), (63, 2), (64, 1), (65, 5), (1000, 64), (1024, 1024),
-                                 (4097, 3), (40000, 17), (40000, 900), (70000, 1)])
+                                 (4096, 700), (4097, 3), (40000, 17), (40000, 900),
+                                 (70000, 1), (300001, 40)])
 def test_plan_groups_tokens_in_order(pkg, T, n, bits):
     g = torch.Generator().manual_seed(T + n)
     ids = torch.randint(-2, n + 2, (T,), generator=g, dtype=torch.int64)
@@ -497,7 +498,7 @@ def test_c_entry_refusals(pkg):
     out = (ctypes.c_uint64 * 3)()
     assert lib.mi_adapter_plan_layout(4, 2, None) == NULL and lib.mi_adapter_plan_layout(4, 0, out) == SHAPE
     assert lib.mi_adapter_plan_layout((1 << 24) + 1, 2, out) == SHAPE and lib.mi_adapter_plan_layout(100, 3, out) == 0
-    assert out[1] + 100 == out[2] and out[2] + 4 == out[0]
+    assert out[1] + 100 == out[2] and out[2] + 4 <= out[0]
     assert lib.mi_adapter_plan(p, 16, 4, 2, p, None) == DTYPE and lib.mi_adapter_plan(p, 32, 4, 1025, p, None) == SHAPE
     assert lib.mi_adapter_plan(None, 32, 4, 2, p, None) == NULL and lib.mi_adapter_plan(p, 32, 4, 2, None, None) == NULL
     assert lib.mi_adapter_plan(p, 32, 4, 2, p + 4, None) == ALIGN and lib.mi_adapter_plan(p + 4, 64, 4, 2, p, None) == ALIGN
