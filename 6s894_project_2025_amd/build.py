@@ -62,6 +62,8 @@ ISA_CHECKED = {"fused_gemm_xreg.hip", "fused_gemm_xreg_f32.hip", "fused_gemm_xre
 # Files whose MFMAs are the compiler's own but which use the direct global -> LDS transfers (M0 is
 # theirs alone) and wait for them by hand before ordinary LDS reads: the M0 and LDS-read checks only.
 TRANSFER_CHECKED = {"fused_gemv_stream.hip"}
+# Files whose matrix-core instructions stand in wavefront-dependent control flow: the masked-MFMA check.
+MASK_CHECKED = {"lora.hip"}
 _MFMA_B_IN_AGPR = re.compile(r"^\s*v_mfma_\S+\s+v\[[0-9:]+\], v\S+, a")
 _AGPR_WRITE = re.compile(r"^\s*v_accvgpr_(write|mov)")
 _LABEL = re.compile(r"^([A-Za-z_][\w$]*):")
@@ -252,6 +254,29 @@ def check_m0_is_the_transfers_alone(asm_text: str, where: str) -> int:
     return writes
 
 
+def check_no_masked_mfma(asm_text: str, where: str) -> int:
+    """Matrix-core instructions ignore the lane mask.  Where the compiler takes a condition to differ
+    between lanes it may save and narrow EXEC and run the conditional code without a branch around it;
+    an MFMA in there then executes for wavefronts that should have skipped it, and corrupts their
+    accumulators.  Raises if an MFMA stands behind such a narrowing with neither a branch nor a label nor
+    the restoring of EXEC in between; returns the number of MFMAs checked."""
+    checked, name, masked = 0, None, None
+    for line in asm_text.splitlines():
+        text = line.split(";")[0].strip()
+        label = _ANY_LABEL.match(text)
+        if label:
+            name, masked = (label.group(1), None) if not label.group(1).startswith(".") else (name, None)
+        elif text.startswith("s_and_saveexec"):
+            masked = text
+        elif text.startswith(("s_cbranch", "s_branch", "s_or_b64 exec", "s_mov_b64 exec")):
+            masked = None
+        elif text.startswith("v_mfma"):
+            checked += 1
+            if masked:
+                raise RuntimeError(f"{where}: {name}: `{text}` executes whatever `{masked}` leaves of the wavefront")
+    return checked
+
+
 _LGKM_WAIT = re.compile(r"lgkmcnt\((\d+)\)")
 kLdsReadHorizon = 400  # instructions followed per path; a fragment is used within a few K steps
 
@@ -335,15 +360,16 @@ def _compile(src: str) -> str:
     obj = os.path.join(OBJ_DIR, base[:-4] + ".o")
     checked = base in ISA_CHECKED
     transfers = base in TRANSFER_CHECKED
+    masks = base in MASK_CHECKED
     cmd = [_hipcc(), *HIPCC_FLAGS, *PER_FILE_FLAGS.get(base, []),
-           *(["-save-temps=obj"] if checked or transfers else []), "-c", src, "-o", obj]
+           *(["-save-temps=obj"] if checked or transfers or masks else []), "-c", src, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     err = "\n".join(l for l in r.stderr.splitlines() if "recognized feature" not in l)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed on {src}:\n{err}")
     if err.strip():
         sys.stderr.write(err + "\n")
-    if checked or transfers:
+    if checked or transfers or masks:
         temps = glob.glob(os.path.join(OBJ_DIR, base[:-4] + "-*")) + glob.glob(os.path.join(OBJ_DIR, base + "-*"))
         isa = [t for t in temps if t.endswith(f"{ARCH}.s")]
         if len(isa) != 1:
@@ -353,10 +379,13 @@ def _compile(src: str) -> str:
         if checked and (check_register_resident_isa(text, base) == 0 or
                         check_mfma_results_not_touched_early(text, base) == 0):
             raise RuntimeError(f"{base}: no register-resident MFMA loop found in the device assembly")
-        if check_m0_is_the_transfers_alone(text, base) == 0:
-            raise RuntimeError(f"{base}: no global -> LDS transfer found in the device assembly")
-        if check_lds_reads_waited_for(text, base) == 0:
-            raise RuntimeError(f"{base}: no LDS read found in the device assembly")
+        if not masks:
+            if check_m0_is_the_transfers_alone(text, base) == 0:
+                raise RuntimeError(f"{base}: no global -> LDS transfer found in the device assembly")
+            if check_lds_reads_waited_for(text, base) == 0:
+                raise RuntimeError(f"{base}: no LDS read found in the device assembly")
+        elif check_no_masked_mfma(text, base) == 0:
+            raise RuntimeError(f"{base}: no MFMA found in the device assembly")
         if checked:
             check_mfma_operands_not_overwritten_early(text, base)
         for t in temps:

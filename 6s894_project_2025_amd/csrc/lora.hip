@@ -1256,6 +1256,7 @@ extern "C" int mi_lora_add(const void* y, const void* x, const void* A, const vo
     if (!aligned16(y) || !aligned16(x) || !aligned16(A) || !aligned16(B) || !aligned16(plan) || !aligned16(out) || !aligned16(workspace) ||
         reinterpret_cast<uintptr_t>(scales) & 3u || reinterpret_cast<uintptr_t>(shrunk) & 3u)
         return MI_ERR_ALIGN;
+    if (d->tokens > 1u && d->out_stride < d->N) return MI_ERR_SHAPE;  // rows that overlap
     if (y == out && d->y_stride != d->out_stride && d->tokens > 1u) return MI_ERR_ALIAS;
     hipStream_t s = static_cast<hipStream_t>(stream);
     unsigned char* ws = static_cast<unsigned char*>(workspace);
@@ -1277,6 +1278,7 @@ extern "C" int mi_lora_add_backward(const void* dy, const void* x, const void* A
         !aligned16(dA) || !aligned16(dB) || !aligned16(workspace) || reinterpret_cast<uintptr_t>(scales) & 3u ||
         reinterpret_cast<uintptr_t>(shrunk) & 3u)
         return MI_ERR_ALIGN;
+    if (d->tokens > 1u && d->out_stride < d->K) return MI_ERR_SHAPE;
     hipStream_t s = static_cast<hipStream_t>(stream);
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     if (d->dtype == MI_F32) return backward<float>(d, dy, x, A, B, scales, plan, shrunk, dx_in, dx, dA, dB, ws, s);

@@ -642,6 +642,9 @@ int make_args(const mi_heads* d, const void* const* tensors, int count, const vo
     for (int i = 0; i < count; ++i) {
         if ((i & 1 ? d->k_heads : d->q_heads) == 0) continue;
         if (!tensors[i]) return MI_ERR_NULL;
+        // outputs whose heads would overlap
+        if (i >= count - 2 && ((d->tokens > 1u && d->token_stride[i] < a.D) || ((i & 1 ? d->k_heads : d->q_heads) > 1u && d->head_stride[i] < a.D)))
+            return MI_ERR_SHAPE;
         if (!aligned16(tensors[i]) || d->token_stride[i] % unit || d->head_stride[i] % unit) return MI_ERR_ALIGN;
     }
     if (a.R && (!positions || !inv_freq)) return MI_ERR_NULL;

@@ -470,7 +470,7 @@ def test_c_entry_refusals(pkg):
     DTYPE, SIZE, ALIGN, NULL, SHAPE, _, ALIAS = range(-1, -8, -1)
     p, q = 1 << 20, 1 << 21  # never followed: every call is refused or has nothing to do
 
-    def sizes(T=4, xs=32, ys=24, os=24, n=2, r=8, K=32, N=24, dt=1):
+    def sizes(T=4, xs=32, ys=24, os=32, n=2, r=8, K=32, N=24, dt=1):
         return pack(T, xs, ys, os, n, r, K, N, dt)
 
     def fwd(d, y=p, x=p, scales=None, plan=p, out=q, shrunk=None, ws=p):
@@ -486,13 +486,14 @@ def test_c_entry_refusals(pkg):
             assert f(sizes(**bad)) == SHAPE, bad
             assert lib.mi_lora_workspace(sizes(**bad), 0) == 0
         assert f(sizes(xs=33)) == ALIGN and f(sizes(ys=28)) == ALIGN and f(sizes(os=26)) == ALIGN
-        assert f(sizes(xs=36, ys=28, os=28, dt=0), plan=None) == NULL
+        assert f(sizes(xs=36, ys=28, os=36, dt=0), plan=None) == NULL
         for bad in ("y", "x", "plan", "out", "ws"):
             assert f(sizes(), **{bad: None}) == NULL, bad
             assert f(sizes(), **{bad: p + 8}) == ALIGN, bad
         assert f(sizes(), scales=p + 2) == ALIGN and f(sizes(), shrunk=p + 2) == ALIGN
+    assert fwd(sizes(os=16)) == SHAPE and bwd(sizes(os=24)) == SHAPE  # rows of the output would overlap
     assert fwd(sizes(T=0), y=None) == 0
-    assert fwd(sizes(ys=32), y=p, out=p) == ALIAS
+    assert fwd(sizes(ys=24), y=p, out=p) == ALIAS
     assert lib.mi_lora_workspace(sizes(), 0) > 0 and lib.mi_lora_workspace(sizes(), 1) > lib.mi_lora_workspace(sizes(), 0)
     assert lib.mi_lora_workspace(None, 0) == 0
     out = (ctypes.c_uint64 * 3)()

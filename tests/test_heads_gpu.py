@@ -420,7 +420,7 @@ def test_c_entry_refusals(pkg):
     DTYPE, SIZE, ALIGN, NULL, SHAPE = range(-1, -6, -1)
     p = 1 << 20  # an address that is never followed: every call is refused, or has nothing to do
 
-    def desc(T=4, ts=(128, 64, 128, 64, 0, 0), hs=(64,) * 6, Hq=2, Hk=1, D=64, R=64, axes=1, ends=(32, 0, 0, 0),
+    def desc(T=4, ts=(128, 64, 128, 64, 128, 64), hs=(64,) * 6, Hq=2, Hk=1, D=64, R=64, axes=1, ends=(32, 0, 0, 0),
              dt=1, wdt=1, pb=32, fb=32, flags=0, eps=1e-6):
         return heads._HEADS.pack(T, *ts, *hs, Hq, Hk, D, R, axes, *ends, dt, wdt, pb, fb, flags, eps)
 
@@ -444,7 +444,8 @@ def test_c_entry_refusals(pkg):
         assert f(desc(Hq=65537)) == SHAPE and f(desc(T=1 << 40)) == SHAPE
         assert f(desc(), q=None) == NULL and f(desc(), pos=None) == NULL
         assert f(desc(), q=p + 2) == ALIGN
-        assert f(desc(ts=(129, 64, 128, 64, 0, 0))) == ALIGN and f(desc(hs=(64, 65, 64, 64, 0, 0))) == ALIGN
+        assert f(desc(ts=(128, 64, 48, 64, 48, 64))) == SHAPE and f(desc(hs=(64, 64, 0, 64, 0, 64))) == SHAPE  # outputs overlap
+        assert f(desc(ts=(129, 64, 128, 64, 128, 64))) == ALIGN and f(desc(hs=(64, 65, 64, 64, 64, 64))) == ALIGN
     assert call(desc(), w=p + 2) == ALIGN and back(desc(), ws=None) == NULL and back(desc(), ws=p + 4) == ALIGN
     assert call(desc(T=0), q=None) == 0 and call(desc(Hq=0, Hk=0), q=None) == 0
     assert lib.mi_qk_norm_rope_workspace(0, 64) == 0
