@@ -1046,9 +1046,11 @@ int check(const mi_lora* d)
     return MI_OK;
 }
 
-// How a batch is cut.  With few tokens for each adapter (16 on the average, or 256 in all) workgroups take 16
-// tokens instead of 64, and their wavefronts different parts of the adapter, which is then most of what
-// there is to read; and the expansion adds up the parts of P itself, a launch less.
+// How a batch is cut.  With at most 16 tiles workgroups take 16 tokens instead of 64, their wavefronts take
+// different parts of the adapter, which is then most of what there is to read, and the expansion adds up the
+// parts of P itself, a launch less (rank 16, 4096 -> 4096, one token 6.7 us against 8.5, 64 tokens of four
+// adapters 7.1 against 9.5).  With more tiles the four times as many workgroups cost more than that (64
+// tokens of 48 adapters, 4096 -> 14336: 17 us against 13.6).
 struct Cut {
     bool few;
     uint32_t rp, splits, parts;
@@ -1056,7 +1058,7 @@ struct Cut {
     Cut(const mi_lora* d, uint32_t K, uint32_t N)
     {
         max_tiles = PlanLayout(d->tokens, d->n_adapters).max_tiles;
-        few = d->tokens <= 256u || d->tokens <= 16u * d->n_adapters;
+        few = max_tiles <= 16u;
         grid_tiles = few ? 4u * max_tiles : max_tiles;
         rp = padded_rank(d->rank);
         const uint32_t block = 16u * elements_of(d->dtype);  // columns of a block, of x and of y
