@@ -26,14 +26,6 @@ namespace mi {
 namespace adapters {
 namespace {
 
-#ifndef WE
-#define WE 2
-#endif
-#ifdef NTL
-#define LOADY(V, p) __builtin_nontemporal_load(reinterpret_cast<const V*>(p))
-#else
-#define LOADY(V, p) load16<V>(p)
-#endif
 constexpr uint32_t kThreads = 256;
 
 // A matrix-core step on 16-byte fragments: lane l holds row (or column) l % 16 and the VEC values of the
@@ -468,7 +460,7 @@ struct ExpandArgs {
     uint64_t out_stride;
     const void* M;       // [n][N][rank]
     const unsigned char* vectors;  // [tiles][Operand::VECTORS], and their
-    const float* down;             // [tiles][64]; not with FEW, which makes them from
+    const float* down;             // [tiles][64]; or NULL, and with OWN they are made from
     const float* scales;           // [n] or NULL
     const float* P;                // [splits][tokens][16 RT], and gives
     float* shrunk;                 // [tokens][rank] or NULL
@@ -482,7 +474,7 @@ struct ExpandArgs {
 // computed.  LIVE: the wavefront has tokens.  Tokens behind the tile's are the first of the 16 again and
 // columns behind N the last VEC: these lanes compute and store what the owner does, from a y that was loaded
 // before the owner stores (out may be y), so that no load or store stands behind a branch.
-template <class E, int RT, bool HAS_Y, bool FEW, bool LIVE>
+template <class E, int RT, bool HAS_Y, bool FEW, bool OWN, bool LIVE>
 __device__ __forceinline__ void expand_blocks(const ExpandArgs& a, const Tile& tile, uint32_t part, unsigned char* lds,
                                               const unsigned char* vectors, const float* down)
 {
@@ -520,7 +512,7 @@ __device__ __forceinline__ void expand_blocks(const ExpandArgs& a, const Tile& t
             d[q] = X::SCALED ? down[at] : 1.0f;
         }
     }
-    if (FEW) __syncthreads();  // the buffers of M take the place of the vectors
+    if (OWN) __syncthreads();  // the buffers of M take the place of the vectors
     if (FEW && !blocks) return;
     unsigned char* const buffer = FEW ? lds + wave * O::BLOCK : lds;
 
@@ -553,7 +545,7 @@ __device__ __forceinline__ void expand_blocks(const ExpandArgs& a, const Tile& t
     auto request_y = [&](V (&to)[4], uint32_t i) __attribute__((always_inline)) {
         if (LIVE && HAS_Y)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) to[q] = LOADY(V, yr[q] + column(i));
+            for (int q = 0; q < 4; ++q) to[q] = load16<V>(yr[q] + column(i));
     };
     auto compute = [&](const unsigned char* from, const V (&y)[4], uint32_t i) __attribute__((always_inline)) {
         if (!LIVE) return;
@@ -610,23 +602,26 @@ __device__ __forceinline__ void expand_blocks(const ExpandArgs& a, const Tile& t
     }
 }
 
-template <class E, int RT, bool HAS_Y, bool FEW>
-__global__ void __launch_bounds__(256, RT == 8 || FEW ? 1 : WE) expand_rows_kernel(ExpandArgs a)
+// OWN: the workgroup makes its tile's vectors from the sums of P itself; otherwise tile_vectors_kernel has.
+template <class E, int RT, bool HAS_Y, bool FEW, bool OWN>
+__global__ void __launch_bounds__(256, RT == 8 || FEW ? 1 : 2) expand_rows_kernel(ExpandArgs a)
 {
     using V = typename Mx<E>::V;
     using O = Operand<E, RT>;
     constexpr uint32_t VEC = Mx<E>::VEC;
     constexpr uint32_t buffers = (FEW ? 4u : 2u) * O::BLOCK;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[FEW && buffers < O::VECTORS ? O::VECTORS : buffers];
-    __shared__ float own_down[FEW ? 16 : 1];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[OWN && buffers < O::VECTORS ? O::VECTORS : buffers];
+    __shared__ float own_down[64];
     const PlanLayout L(a.tokens, a.n);
     Tile tile;
     uint32_t part;
     if (!take_tile<FEW>(a.plan, L, a.parts, tile, part)) return;
     if ((uint32_t)tile.adapter < a.n) {
-        if constexpr (FEW) {
+        const unsigned char* vectors = lds;
+        const float* down = own_down;
+        if constexpr (OWN) {
             const uint32_t t = threadIdx.x >> 2, count = (uint32_t)tile.count;
-            if (t < 16u) {
+            if (!FEW || t < 16u) {
                 const uint64_t position = (uint64_t)(uint32_t)tile.first + source_token(t, count);
                 f32x4 v[RT];
                 sum_parts<RT>(a.P, a.tokens, a.splits, position, v);
@@ -639,14 +634,14 @@ __global__ void __launch_bounds__(256, RT == 8 || FEW ? 1 : WE) expand_rows_kern
                 if (Mx<E>::SCALED && (threadIdx.x & 3u) == 0) own_down[t] = d;
             }
             __syncthreads();
-            expand_blocks<E, RT, HAS_Y, FEW, true>(a, tile, part, lds, lds, own_down);
         } else {
             const uint64_t id = blockIdx.x / a.parts;
-            const unsigned char* vectors = a.vectors + id * O::VECTORS;
-            // every wavefront meets the same barriers on either way
-            if (16u * this_wave() < (uint32_t)tile.count) expand_blocks<E, RT, HAS_Y, FEW, true>(a, tile, part, lds, vectors, a.down + id * 64u);
-            else expand_blocks<E, RT, HAS_Y, FEW, false>(a, tile, part, lds, vectors, a.down + id * 64u);
+            vectors = a.vectors + id * O::VECTORS;
+            down = a.down + id * 64u;
         }
+        // every wavefront meets the same barriers on either way
+        if (FEW || 16u * this_wave() < (uint32_t)tile.count) expand_blocks<E, RT, HAS_Y, FEW, OWN, true>(a, tile, part, lds, vectors, down);
+        else expand_blocks<E, RT, HAS_Y, FEW, OWN, false>(a, tile, part, lds, vectors, down);
         return;
     }
     // tokens without an adapter: y as it is, or zeros
@@ -659,7 +654,7 @@ __global__ void __launch_bounds__(256, RT == 8 || FEW ? 1 : WE) expand_rows_kern
                 __builtin_nontemporal_store(v, reinterpret_cast<V*>(static_cast<E*>(a.out) + t * a.out_stride + c));
             }
         }
-    if (FEW && a.shrunk && part == 0u)
+    if (OWN && a.shrunk && part == 0u)
         for (uint32_t i = threadIdx.x; i < (uint32_t)tile.count * a.rank; i += kThreads) {
             const uint32_t at = i / a.rank;
             a.shrunk[(uint64_t)(uint32_t)a.plan[L.order + (uint32_t)tile.first + at] * a.rank + (i - at * a.rank)] = 0.0f;
@@ -1012,15 +1007,6 @@ uint32_t cut(uint64_t tiles, uint32_t blocks, uint32_t least, uint32_t most)
     return parts > 8u ? parts / 8u * 8u : parts;
 }
 
-#ifndef EB
-#define EB 2u
-#endif
-#ifndef MC
-#define MC 1024u
-#endif
-#ifndef ME
-#define ME 8192u
-#endif
 template <class F>
 void for_rank(uint32_t rp, F f)
 {
@@ -1062,8 +1048,11 @@ struct Cut {
         grid_tiles = few ? 4u * max_tiles : max_tiles;
         rp = padded_rank(d->rank);
         const uint32_t block = 16u * elements_of(d->dtype);  // columns of a block, of x and of y
-        splits = cut(max_tiles, (K + block - 1u) / block, few ? 4u : 2u, MC);
-        parts = cut(max_tiles, (N + block - 1u) / block, few ? 4u : EB, few ? 1024u : ME);
+        // x: the workgroups that run at once.  y: ten times that, as one round and a little of long ones leaves
+        // compute units idle (8192 tokens, N = 14336: 128 us with 1100 workgroups, 100 with 7700), but two
+        // blocks each, so that one is requested while the other is computed (one each: 116 us).
+        splits = cut(max_tiles, (K + block - 1u) / block, few ? 4u : 2u, 1024u);
+        parts = cut(max_tiles, (N + block - 1u) / block, few ? 4u : 2u, few ? 1024u : 8192u);
     }
     uint64_t sums() const { return (uint64_t)splits * rp * 4u; }  // bytes of P per token
 };
@@ -1082,13 +1071,18 @@ uint64_t pieces_bytes(uint32_t rp) { return (uint64_t)rp * 64u * 4u; }  // two o
 
 struct ForwardPlan {
     Cut c;
+    bool own;
     uint64_t P, vectors, down, bytes;
     explicit ForwardPlan(const mi_lora* d) : c(d, d->K, d->N)
     {
+        // a launch less where adding up P again in every workgroup moves no more than 16 MB: 64 tokens of 48
+        // adapters, 4096 -> 14336, rank 16 (4 MB) 18.3 us a call against 22.5, of which the GPU works 16.0 and
+        // 14.6; 512 tokens of 64 adapters, rank 64 (58 MB) 62 against 51
+        own = c.few || c.sums() * d->tokens * c.parts <= 1u << 24;
         Take take;
         P = take(c.sums() * d->tokens);
-        vectors = take(c.few ? 0u : c.max_tiles * pieces_bytes(c.rp));
-        down = take(c.few ? 0u : c.max_tiles * 64u * 4u);
+        vectors = take(own ? 0u : c.max_tiles * pieces_bytes(c.rp));
+        down = take(own ? 0u : c.max_tiles * 64u * 4u);
         bytes = take.end;
     }
 };
@@ -1150,9 +1144,10 @@ int expand(const Cut& c, ExpandArgs a, hipStream_t s)
     const dim3 grid((uint32_t)c.grid_tiles * c.parts);
     for_rank(c.rp, [&](auto rt) {
         constexpr int RT = decltype(rt)::value;
-        if (a.y.p && c.few) hipLaunchKernelGGL((expand_rows_kernel<E, RT, true, true>), grid, dim3(kThreads), 0, s, a);
-        else if (a.y.p) hipLaunchKernelGGL((expand_rows_kernel<E, RT, true, false>), grid, dim3(kThreads), 0, s, a);
-        else hipLaunchKernelGGL((expand_rows_kernel<E, RT, false, false>), grid, dim3(kThreads), 0, s, a);
+        if (!a.y.p) hipLaunchKernelGGL((expand_rows_kernel<E, RT, false, false, false>), grid, dim3(kThreads), 0, s, a);
+        else if (a.vectors) hipLaunchKernelGGL((expand_rows_kernel<E, RT, true, false, false>), grid, dim3(kThreads), 0, s, a);
+        else if (c.few) hipLaunchKernelGGL((expand_rows_kernel<E, RT, true, true, true>), grid, dim3(kThreads), 0, s, a);
+        else hipLaunchKernelGGL((expand_rows_kernel<E, RT, true, false, true>), grid, dim3(kThreads), 0, s, a);
     });
     return launch_status();
 }
@@ -1166,11 +1161,11 @@ int forward(const mi_lora* d, const void* y, const void* x, const void* A, const
     float* down = reinterpret_cast<float*>(ws + f.down);
     int st;
     if ((st = contract<E>(d, plan, {x, d->x_stride}, A, d->K, f.c, P, s)) != MI_OK) return st;
-    if (!f.c.few) {
+    if (!f.own) {
         const VectorArgs v{plan, P, scales, shrunk, ws + f.vectors, down, nullptr, nullptr, d->tokens, d->n_adapters, d->rank, f.c.splits, false};
         if ((st = tile_vectors<E>(f.c, v, s)) != MI_OK) return st;
     }
-    return expand<E>(f.c, {plan, {y, d->y_stride}, out, d->out_stride, B, ws + f.vectors, down, scales, P, shrunk, d->tokens, d->n_adapters,
+    return expand<E>(f.c, {plan, {y, d->y_stride}, out, d->out_stride, B, f.own ? nullptr : ws + f.vectors, down, scales, P, shrunk, d->tokens, d->n_adapters,
                            d->rank, d->N, 0, 0}, s);
 }
 
