@@ -14,8 +14,8 @@
 //   contract_rows   P[split][position][r] = sum over a part of the long axis of row . M[a]:  u, and d / s
 //   expand_rows     out = y + s (sum of P) M'[a]^T:  the forward output, and dx
 //   gradient_rows   dB of up to 512 tokens and P of d, from one pass over g
-//   transpose       A^T of the adapters in use, for dx by expand_rows
-//   tile_vectors    the sums of P times s, split, as operands of expand_rows and, transposed, of weight_rows
+//   tile_vectors    the sums of P times s, split, as operands of expand_rows and, transposed, of weight_rows;
+//                   and A^T of the adapters in use, for dx by expand_rows
 //   weight_rows     dA of up to 512 tokens;  weight_sum adds the weights' parts up
 // All sums are in a fixed order.
 #include <type_traits>
@@ -359,6 +359,25 @@ __device__ __forceinline__ uint32_t source_token(uint32_t t, uint32_t count)
 }
 
 // ------------------------------------------------------------------------------------------------
+// A^T of the adapters in use, for dx: a thread has eight ranks of one k, so that reads are whole lines along k and
+// the stores 16 or 32 bytes of neighbouring rows.
+template <class E>
+__device__ __forceinline__ void transpose_adapters(const int32_t* plan, const PlanLayout& L, const E* A, E* At, uint32_t rank, uint32_t K,
+                                                   uint32_t block)
+{
+    typedef E E4 __attribute__((ext_vector_type(4)));
+    const uint32_t blocks_k = (K + kThreads - 1u) / kThreads, rest = block / blocks_k;
+    const uint32_t k = (block - rest * blocks_k) * kThreads + threadIdx.x, r0 = rest % (rank / 8u) * 8u, ad = rest / (rank / 8u);
+    if (k >= K || plan[L.starts + ad] == plan[L.starts + ad + 1u]) return;
+    const E* src = A + ((uint64_t)ad * rank + r0) * K + k;
+    E4 v[2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = src[(uint64_t)i * K];
+    E4* dst = reinterpret_cast<E4*>(At + ((uint64_t)ad * K + k) * rank + r0);
+    dst[0] = v[0];
+    dst[1] = v[1];
+}
+
 struct VectorArgs {
     const int32_t* plan;
     const float* P;        // [splits][tokens][16 RT]
@@ -371,6 +390,9 @@ struct VectorArgs {
     uint64_t tokens;
     uint32_t n, rank, splits;
     bool given;
+    const void* A;         // NULL, or [n][rank][K]: workgroups behind the tiles' transpose it
+    void* At;              // [n][K][rank]
+    uint32_t K, tiles;     // workgroups of the tiles
 };
 
 // Where a tile is used by many workgroups: its vectors once, from the sums of P (or from the given ones) times
@@ -384,6 +406,8 @@ __global__ void __launch_bounds__(256) tile_vectors_kernel(VectorArgs a)
     __shared__ float top[4];
     __shared__ E turned[RP * X::PIECES * 64u];
     const PlanLayout L(a.tokens, a.n);
+    if (blockIdx.x >= a.tiles)
+        return transpose_adapters<E>(a.plan, L, static_cast<const E*>(a.A), static_cast<E*>(a.At), a.rank, a.K, blockIdx.x - a.tiles);
     const Tile tile = reinterpret_cast<const Tile*>(a.plan)[blockIdx.x];
     if (blockIdx.x >= (uint32_t)a.plan[L.counts]) return;
     const uint32_t t = threadIdx.x >> 2, r0 = (threadIdx.x & 3u) * 4u * RT, count = (uint32_t)tile.count;
@@ -659,33 +683,6 @@ __global__ void __launch_bounds__(256, RT == 8 || FEW ? 1 : 2) expand_rows_kerne
             const uint32_t at = i / a.rank;
             a.shrunk[(uint64_t)(uint32_t)a.plan[L.order + (uint32_t)tile.first + at] * a.rank + (i - at * a.rank)] = 0.0f;
         }
-}
-
-// ------------------------------------------------------------------------------------------------
-struct TransposeArgs {
-    const int32_t* plan;
-    const void* src;     // A [n][rank][K]
-    void* dst;           // [n][K][rank]
-    uint64_t tokens;
-    uint32_t n, rank, K;
-};
-
-// A^T of the adapters in use: a thread has eight ranks of one k, so that reads are whole lines along k and the
-// stores 16 or 32 bytes of the neighbouring rows.
-template <class E>
-__global__ void __launch_bounds__(256) transpose_kernel(TransposeArgs a)
-{
-    const PlanLayout L(a.tokens, a.n);
-    const uint32_t k = blockIdx.x * kThreads + threadIdx.x, r0 = 8u * blockIdx.y, ad = blockIdx.z;
-    if (k >= a.K || a.plan[L.starts + ad] == a.plan[L.starts + ad + 1u]) return;
-    const E* src = static_cast<const E*>(a.src) + ((uint64_t)ad * a.rank + r0) * a.K + k;
-    typedef E E4 __attribute__((ext_vector_type(4)));
-    E4 v[2];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = src[(uint64_t)i * a.K];
-    E4* dst = reinterpret_cast<E4*>(static_cast<E*>(a.dst) + ((uint64_t)ad * a.K + k) * a.rank + r0);
-    dst[0] = v[0];
-    dst[1] = v[1];
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1128,10 +1125,12 @@ int contract(const mi_lora* d, const int32_t* plan, Rows x, const void* M, uint3
 }
 
 template <class E>
-int tile_vectors(const Cut& c, const VectorArgs& a, hipStream_t s)
+int tile_vectors(const Cut& c, VectorArgs a, hipStream_t s)
 {
+    a.tiles = (uint32_t)c.max_tiles;
+    const uint32_t more = a.A ? (a.K + kThreads - 1u) / kThreads * (a.rank / 8u) * a.n : 0u;
     for_rank(c.rp, [&](auto rt) {
-        hipLaunchKernelGGL((tile_vectors_kernel<E, decltype(rt)::value>), dim3((uint32_t)c.max_tiles), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL((tile_vectors_kernel<E, decltype(rt)::value>), dim3(a.tiles + more), dim3(kThreads), 0, s, a);
     });
     return launch_status();
 }
@@ -1162,7 +1161,7 @@ int forward(const mi_lora* d, const void* y, const void* x, const void* A, const
     int st;
     if ((st = contract<E>(d, plan, {x, d->x_stride}, A, d->K, f.c, P, s)) != MI_OK) return st;
     if (!f.own) {
-        const VectorArgs v{plan, P, scales, shrunk, ws + f.vectors, down, nullptr, nullptr, d->tokens, d->n_adapters, d->rank, f.c.splits, false};
+        const VectorArgs v{plan, P, scales, shrunk, ws + f.vectors, down, nullptr, nullptr, d->tokens, d->n_adapters, d->rank, f.c.splits, false, nullptr, nullptr, 0, 0};
         if ((st = tile_vectors<E>(f.c, v, s)) != MI_OK) return st;
     }
     return expand<E>(f.c, {plan, {y, d->y_stride}, out, d->out_stride, B, f.own ? nullptr : ws + f.vectors, down, scales, P, shrunk, d->tokens, d->n_adapters,
@@ -1180,9 +1179,9 @@ int backward(const mi_lora* d, const void* dy, const void* x, const void* A, con
     const Rows rx{x, d->x_stride}, rdy{dy, d->y_stride};
     int st;
     if (d->tokens) {
-        // s u, transposed
+        // s u, transposed, and A^T
         VectorArgs v{plan, P, scales, const_cast<float*>(shrunk), nullptr, nullptr, ws + b.pieces[1], tile_down[1],
-                     d->tokens, d->n_adapters, d->rank, b.u.splits, shrunk != nullptr};
+                     d->tokens, d->n_adapters, d->rank, b.u.splits, shrunk != nullptr, A, ws + b.at, d->K, 0};
         if (!shrunk && (st = contract<E>(d, plan, rx, A, d->K, b.u, P, s)) != MI_OK) return st;
         if ((st = tile_vectors<E>(b.c, v, s)) != MI_OK) return st;
         const PlanLayout L(d->tokens, d->n_adapters);
@@ -1200,6 +1199,7 @@ int backward(const mi_lora* d, const void* dy, const void* x, const void* A, con
             hipLaunchKernelGGL((gradient_rows_kernel<E, decltype(r)::value>), grid, dim3(kThreads), 0, s, w);
         });
         if (st != MI_OK) return st;
+        v.A = nullptr;
         v.shrunk = nullptr;
         v.given = false;
         v.splits = b.slices;
@@ -1209,9 +1209,6 @@ int backward(const mi_lora* d, const void* dy, const void* x, const void* A, con
         v.tile_down = tile_down[0];
         if ((st = tile_vectors<E>(b.c, v, s)) != MI_OK) return st;
         // dx
-        TransposeArgs t{plan, A, ws + b.at, d->tokens, d->n_adapters, d->rank, d->K};
-        hipLaunchKernelGGL((transpose_kernel<E>), dim3((d->K + kThreads - 1u) / kThreads, d->rank / 8u, d->n_adapters), dim3(kThreads), 0, s, t);
-        if ((st = launch_status()) != MI_OK) return st;
         if ((st = expand<E>(b.c, {plan, {dx_in, d->out_stride}, dx, d->out_stride, ws + b.at, ws + b.vectors, down, nullptr, nullptr, nullptr,
                                   d->tokens, d->n_adapters, d->rank, d->K, 0, 0}, s)) != MI_OK)
             return st;
@@ -1276,6 +1273,8 @@ extern "C" int mi_lora_add_backward(const void* dy, const void* x, const void* A
         reinterpret_cast<uintptr_t>(shrunk) & 3u)
         return MI_ERR_ALIGN;
     if (d->tokens > 1u && d->out_stride < d->K) return MI_ERR_SHAPE;
+    // A^T is made by a workgroup for every 2048 values, in one grid with the tiles: below 2^32 threads
+    if ((uint64_t)d->n_adapters * d->rank * ((d->K + 255u) / 256u * 256u) >= 1ull << 35) return MI_ERR_SHAPE;
     hipStream_t s = static_cast<hipStream_t>(stream);
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     if (d->dtype == MI_F32) return backward<float>(d, dy, x, A, B, scales, plan, shrunk, dx_in, dx, dA, dB, ws, s);

@@ -186,6 +186,7 @@ int mi_lora_add(const void* y, const void* x, const void* A, const void* B, cons
  *   shrunk    : u from the forward pass, or NULL (it is computed again from x).
  *   dx_in     : NULL for zeros, or added; may be dx (in place).
  *   workspace : mi_lora_workspace(sizes, 1) bytes.  Outputs overlap no input but dx_in = dx.
+ * A holds fewer than 2^35 values (K rounded up to a multiple of 256), or MI_ERR_SHAPE.
  */
 int mi_lora_add_backward(const void* dy, const void* x, const void* A, const void* B, const float* scales,
                          const int32_t* plan, const float* shrunk, const void* dx_in, void* dx, void* dA,

@@ -491,6 +491,7 @@ def test_c_entry_refusals(pkg):
             assert f(sizes(), **{bad: None}) == NULL, bad
             assert f(sizes(), **{bad: p + 8}) == ALIGN, bad
         assert f(sizes(), scales=p + 2) == ALIGN and f(sizes(), shrunk=p + 2) == ALIGN
+    assert bwd(sizes(n=1024, r=128, K=1 << 18, xs=1 << 18, os=1 << 18)) == SHAPE  # 2^35 values of A
     assert fwd(sizes(os=16)) == SHAPE and bwd(sizes(os=24)) == SHAPE  # rows of the output would overlap
     assert fwd(sizes(T=0), y=None) == 0
     assert fwd(sizes(ys=24), y=p, out=p) == ALIAS
