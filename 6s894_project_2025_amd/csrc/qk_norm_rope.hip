@@ -648,6 +648,8 @@ int make_args(const mi_heads* d, const void* const* tensors, int count, const vo
         if (!aligned16(tensors[i]) || d->token_stride[i] % unit || d->head_stride[i] % unit) return MI_ERR_ALIGN;
     }
     if (a.R && (!positions || !inv_freq)) return MI_ERR_NULL;
+    if (a.R && (reinterpret_cast<uintptr_t>(positions) % (d->position_bits / 8u) || reinterpret_cast<uintptr_t>(inv_freq) % (d->freq_bits / 8u)))
+        return MI_ERR_ALIGN;
     for (int kind = 0; kind < 2; ++kind) {
         const int out = count - 2 + kind;
         Side& side = kind ? a.k : a.q;

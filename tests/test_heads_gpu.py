@@ -443,7 +443,7 @@ def test_c_entry_refusals(pkg):
         assert f(desc(eps=-1.0)) == SHAPE and f(desc(eps=float("nan"))) == SHAPE
         assert f(desc(Hq=65537)) == SHAPE and f(desc(T=1 << 40)) == SHAPE
         assert f(desc(), q=None) == NULL and f(desc(), pos=None) == NULL
-        assert f(desc(), q=p + 2) == ALIGN
+        assert f(desc(), q=p + 2) == ALIGN and f(desc(), pos=p + 2) == ALIGN and f(desc(pb=64), pos=p + 4) == ALIGN
         assert f(desc(ts=(128, 64, 48, 64, 48, 64))) == SHAPE and f(desc(hs=(64, 64, 0, 64, 0, 64))) == SHAPE  # outputs overlap
         assert f(desc(ts=(129, 64, 128, 64, 128, 64))) == ALIGN and f(desc(hs=(64, 65, 64, 64, 64, 64))) == ALIGN
     assert call(desc(), w=p + 2) == ALIGN and back(desc(), ws=None) == NULL and back(desc(), ws=p + 4) == ALIGN
