@@ -21,6 +21,10 @@
 // them where there are few tokens.  A wavefront computes the sines and cosines of its token once (one angle
 // per lane, exchanged through LDS that no other wavefront uses, so there is no barrier) and keeps requests
 // for the next items, of its next tokens too, in flight.
+//
+// Bound: memory.  8192 tokens of 32 + 8 heads of 128 in bf16, out of packed rows, with the Hadamard rotation: 168 MB
+// in 32.5 us (5.2 TB/s; a copy of 512 MB runs at 5.4), 2 us of it the rotation; the backward pass 252 MB in 54 us
+// (4.7 TB/s), 4 us of it the sums of the weight gradients.
 #include <type_traits>
 
 #include "common.hpp"
@@ -93,6 +97,9 @@ __device__ __forceinline__ void unpack_units(const Raw<E> (&r)[2], float (&v)[2]
     }
 }
 
+// Streaming stores: what a pass over a large batch writes is not read again before it would be evicted, and the
+// heads of 8192 tokens took 34.5 us with them against 41.6.  Not for fp32, where one instruction writes every
+// other 16 bytes of a line: 4096 tokens took 62 us with them against 43.
 template <class E>
 __device__ __forceinline__ void store_unit(E* p, const float (&v)[8])
 {
