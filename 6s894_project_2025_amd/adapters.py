@@ -182,7 +182,7 @@ def lora_add_backward(dy: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: tor
     """Gradients of :func:`lora_add`: ``(dx, dA, dB)`` from ``dy``, the gradient of ``out`` (the gradient of ``y``
     is ``dy`` itself).  ``shrunk`` is what the forward call returned with ``return_shrunk``; without it
     ``A[a] @ x[t]`` is computed again.  With ``dx`` given (the shared projection's own gradient) the
-    adapters' part is added to it in place; without, a new tensor with zeros for tokens without an
+    adapters' part is added to it in place (it may be ``x`` itself); without, a new tensor with zeros for tokens without an
     adapter.  ``dA`` and ``dB`` are in the adapters' dtype, zeros for adapters that no token uses; sums
     over tokens are fp32 in a fixed order.
     """

@@ -1208,10 +1208,6 @@ int backward(const mi_lora* d, const void* dy, const void* x, const void* A, con
         v.pieces = ws + b.pieces[0];
         v.tile_down = tile_down[0];
         if ((st = tile_vectors<E>(b.c, v, s)) != MI_OK) return st;
-        // dx
-        if ((st = expand<E>(b.c, {plan, {dx_in, d->out_stride}, dx, d->out_stride, ws + b.at, ws + b.vectors, down, nullptr, nullptr, nullptr,
-                                  d->tokens, d->n_adapters, d->rank, d->K, 0, 0}, s)) != MI_OK)
-            return st;
         // dA
         w.rows = rx;
         w.pieces = ws + b.pieces[0];
@@ -1222,6 +1218,10 @@ int backward(const mi_lora* d, const void* dy, const void* x, const void* A, con
             hipLaunchKernelGGL((weight_rows_kernel<E, decltype(r)::value>), grid, dim3(kThreads), 0, s, w);
         });
         if (st != MI_OK) return st;
+        // dx, after dA: it may lie in x
+        if ((st = expand<E>(b.c, {plan, {dx_in, d->out_stride}, dx, d->out_stride, ws + b.at, ws + b.vectors, down, nullptr, nullptr, nullptr,
+                                  d->tokens, d->n_adapters, d->rank, d->K, 0, 0}, s)) != MI_OK)
+            return st;
     }
     WeightSumArgs sum{plan, reinterpret_cast<float*>(ws + b.partials), {dA, dB}, d->tokens, d->n_adapters, d->rank, {d->K, d->N}};
     hipLaunchKernelGGL((weight_sum_kernel<E>), dim3(512, d->n_adapters), dim3(kThreads), 0, s, sum);

@@ -185,7 +185,8 @@ int mi_lora_add(const void* y, const void* x, const void* A, const void* B, cons
  * in a fixed order; dA, dB are shaped like A, B, zeros for adapters without tokens.
  *   shrunk    : u from the forward pass, or NULL (it is computed again from x).
  *   dx_in     : NULL for zeros, or added; may be dx (in place).
- *   workspace : mi_lora_workspace(sizes, 1) bytes.  Outputs overlap no input but dx_in = dx.
+ *   workspace : mi_lora_workspace(sizes, 1) bytes.  Outputs overlap no input, but dx may lie on dx_in (at
+ *               the same address) and on x, which is read before dx is written.
  * A holds fewer than 2^35 values (K rounded up to a multiple of 256), or MI_ERR_SHAPE.
  */
 int mi_lora_add_backward(const void* dy, const void* x, const void* A, const void* B, const float* scales,

@@ -504,3 +504,23 @@ def test_c_entry_refusals(pkg):
     assert lib.mi_adapter_plan(p, 16, 4, 2, p, None) == DTYPE and lib.mi_adapter_plan(p, 32, 4, 1025, p, None) == SHAPE
     assert lib.mi_adapter_plan(None, 32, 4, 2, p, None) == NULL and lib.mi_adapter_plan(p, 32, 4, 2, None, None) == NULL
     assert lib.mi_adapter_plan(p, 32, 4, 2, p + 4, None) == ALIGN and lib.mi_adapter_plan(p + 4, 64, 4, 2, p, None) == ALIGN
+
+
+# ---------------------------------------------------------------------------------------------
+# calls at the edge of what is allowed
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_input_gradient_written_over_the_input(pkg, dtype):
+    """``dx`` may be ``x`` itself: dA is of the input as it was."""
+    T, n, r, K, N = 300, 2, 16, 264, 136
+    c = make(T, n, r, K, N, dtype, "mixed", seed=12)
+    d = on_gpu(c)
+    plan = pkg.adapter_plan(d["ids"], n)
+    args = (d["A"], d["B"], plan, d["scales"])
+    want = pkg.lora_add_backward(d["dy"], d["x"], *args, dx=d["x"].clone())
+    x = d["x"].clone()
+    got = pkg.lora_add_backward(d["dy"], x, *args, dx=x)
+    assert got[0] is x
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
