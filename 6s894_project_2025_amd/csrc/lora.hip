@@ -13,11 +13,19 @@
 // Tokens come grouped by adapter (adapter_plan.hpp), in tiles of up to 64 of one adapter.
 //   contract_rows   P[split][position][r] = sum over a part of the long axis of row . M[a]:  u, and d / s
 //   expand_rows     out = y + s (sum of P) M'[a]^T:  the forward output, and dx
-//   gradient_rows   dB of up to 512 tokens and P of d, from one pass over g
+//   gradient_rows   dB of a chunk of tokens and P of d, from one pass over g
 //   tile_vectors    the sums of P times s, split, as operands of expand_rows and, transposed, of weight_rows;
 //                   and A^T of the adapters in use, for dx by expand_rows
-//   weight_rows     dA of up to 512 tokens;  weight_sum adds the weights' parts up
+//   weight_rows     dA of a chunk of tokens;  weight_sum adds the weights' parts up
 // All sums are in a fixed order.
+//
+// Bound: HBM.  A rank of 16 is 16 products a value of x and 32 (two pieces) a value of y, far below what
+// the matrix cores do in the time of reading it, so each kernel is one pass over a long matrix, and only the
+// rank-space vectors (rank * 4 bytes a token and part) go between them.  8192 tokens of 8 adapters, 4096 ->
+// 14336, bf16, rank 16: contract_rows 21 us (67 MB), tile_vectors 5, expand_rows 100 (470 MB, 4.7 TB/s: a
+// plain copy of 4 GB reaches 4.7, of 512 MB 5.4).  Backward of 4 adapters: tile_vectors 5 and 5, gradient_rows
+// 50 (235 MB), weight_rows 16, expand_rows 15, weight_sum 6.  Few tokens are bound by their launches
+// (one token: two of 3 us).
 #include <type_traits>
 
 #include "adapter_plan.hpp"
@@ -131,7 +139,7 @@ __device__ __forceinline__ bool take_tile(const int32_t* plan, const PlanLayout&
 
 // P^T tile = M (rows: r) . x^T (columns: tokens), in blocks of 256 bytes of every row, which is how x and M are
 // read (16 lanes a row) on their way into LDS; there the 16-byte pieces of row i are permuted by i, so that 16
-// rows' pieces of one column come from 16 different banks groups.  The workgroup's wavefronts take 16 tokens
+// rows' pieces of one column come from 16 different groups of banks.  The workgroup's wavefronts take 16 tokens
 // each and share the block of M, which has two buffers; with FEW they take every fourth block for the same 16
 // tokens, each with its own M, and add up at the end.  The next block is requested before the present one is
 // computed.  Columns behind the tile's tokens repeat the first of the 16 and rows behind the rank the first
@@ -483,10 +491,12 @@ struct ExpandArgs {
     void* out;
     uint64_t out_stride;
     const void* M;       // [n][N][rank]
-    const unsigned char* vectors;  // [tiles][Operand::VECTORS], and their
-    const float* down;             // [tiles][64]; or NULL, and with OWN they are made from
+    // either: the tiles' vectors, and what undoes their scaling
+    const unsigned char* vectors;  // [tiles][Operand::VECTORS], NULL with OWN
+    const float* down;             // [tiles][64]
+    // or, with OWN: what they are made from, and u as an output
     const float* scales;           // [n] or NULL
-    const float* P;                // [splits][tokens][16 RT], and gives
+    const float* P;                // [splits][tokens][16 RT]
     float* shrunk;                 // [tokens][rank] or NULL
     uint64_t tokens;
     uint32_t n, rank, N, splits, parts;  // workgroup `part` takes every parts-th block of N
@@ -863,7 +873,8 @@ __global__ void __launch_bounds__(256) weight_rows_kernel(WeightArgs a)
 // 16 VEC of the columns and all tokens, STEP at a time with the next requested.  For dB the lanes' registers
 // are turned over as above; for d the same registers go through LDS to become operands along the columns, B
 // stays in registers, and the four wavefronts' sums of a step meet in LDS (two buffers, one barrier a step).
-template <class E, int RT>
+// STREAM: dy is read past the caches (kStreamed).
+template <class E, int RT, bool STREAM>
 __global__ void __launch_bounds__(256, RT == 2 ? 1 : 2) gradient_rows_kernel(WeightArgs a)
 {
     using X = Mx<E>;
@@ -902,7 +913,8 @@ __global__ void __launch_bounds__(256, RT == 2 ? 1 : 2) gradient_rows_kernel(Wei
 #pragma unroll
         for (uint32_t i = 0; i < VEC; ++i) {
             const uint32_t t = t0 + VEC * g + i;
-            in[i] = load16<u32x4>(rows + (uint64_t)(uint32_t)order[t < count ? t : count - 1u] * a.rows.stride);
+            const E* p = rows + (uint64_t)(uint32_t)order[t < count ? t : count - 1u] * a.rows.stride;
+            in[i] = STREAM ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)) : load16<u32x4>(p);
         }
     };
     auto work = [&](u32x4 (&in)[VEC], uint32_t t0, uint32_t buffer) __attribute__((always_inline)) {
@@ -1054,6 +1066,10 @@ struct Cut {
     uint64_t sums() const { return (uint64_t)splits * rp * 4u; }  // bytes of P per token
 };
 
+// From so many bytes of dy on it is read past the caches, a quarter of the last of which it would fill (rank 16:
+// 235 MB 97 us a call against 102, 67 MB 69 against 74; but 59 MB 48.4 against 45.9, 29 MB 38.5 against 35).
+constexpr uint64_t kStreamed = 64u << 20;
+
 struct Take {  // places in a workspace
     uint64_t end = 0;
     uint64_t operator()(uint64_t bytes)
@@ -1196,7 +1212,9 @@ int backward(const mi_lora* d, const void* dy, const void* x, const void* A, con
         WeightArgs w{plan, rdy, ws + b.pieces[1], tile_down[1], partials, dB, B, P, d->tokens, d->n_adapters, d->rank, b.c.rp, d->K, d->N};
         dim3 grid(b.slices, (uint32_t)L.max_chunks, b.c.rp / rt);
         st = for_weights([&](auto r) {
-            hipLaunchKernelGGL((gradient_rows_kernel<E, decltype(r)::value>), grid, dim3(kThreads), 0, s, w);
+            constexpr int RT = decltype(r)::value;
+            if (d->tokens * d->N * sizeof(E) >= kStreamed) hipLaunchKernelGGL((gradient_rows_kernel<E, RT, true>), grid, dim3(kThreads), 0, s, w);
+            else hipLaunchKernelGGL((gradient_rows_kernel<E, RT, false>), grid, dim3(kThreads), 0, s, w);
         });
         if (st != MI_OK) return st;
         v.A = nullptr;

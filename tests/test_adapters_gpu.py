@@ -524,3 +524,17 @@ def test_input_gradient_written_over_the_input(pkg, dtype):
     assert got[0] is x
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,n,r,K,N,dtype,ids", [(4200, 3, 16, 72, 8200, "bf16", "runs"), (4200, 3, 40, 72, 8200, "fp16", "mixed"),
+                                                 (4200, 2, 8, 72, 4104, "fp32", "mixed")])
+def test_backward_of_an_output_larger_than_the_caches_keep(pkg, T, n, r, K, N, dtype, ids):
+    c = make(T, n, r, K, N, dtype, ids, seed=T + r)
+    d = on_gpu(c)
+    plan = pkg.adapter_plan(d["ids"], n)
+    got = pkg.lora_add_backward(d["dy"], d["x"], d["A"], d["B"], plan, d["scales"])
+    gx, dA, dB, gx_slack, dA_slack, dB_slack = backward64(c, dtype)
+    within(got[0], gx, gx_slack, "dx")
+    within(got[1], dA, dA_slack, "dA")
+    within(got[2], dB, dB_slack, "dB")
