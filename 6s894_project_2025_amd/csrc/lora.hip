@@ -815,6 +815,21 @@ __device__ __forceinline__ void store_weights(const WeightArgs& a, const Chunk& 
     }
 }
 
+// The slice of columns and the ranks of workgroup blockIdx.x, of the grid's `slices` rounded up to eights with
+// several `halves` of the ranks: these read the same rows, and eight apart they run on one XCD soon after each
+// other, where the second finds them in L2.
+struct Share {
+    uint32_t slice, half;
+};
+
+__device__ __forceinline__ Share share(uint32_t halves)
+{
+    const uint32_t group = blockIdx.x / (8u * halves), in = blockIdx.x - group * 8u * halves;
+    return halves == 1u ? Share{blockIdx.x, 0u} : Share{group * 8u + (in & 7u), in >> 3};
+}
+
+uint32_t shares(uint32_t slices, uint32_t halves) { return halves == 1u ? slices : (slices + 7u) / 8u * 8u * halves; }
+
 // dA.  Workgroup: a chunk of tokens of one adapter, 16 VEC columns of x, RT * 16 ranks (32 at most: with 64 the
 // registers leave one wavefront per SIMD: a backward pass of 8192 tokens, 4096 -> 4096, rank 64 took 130 us
 // against 109, though rows are then read once less).  A wavefront takes
@@ -834,7 +849,9 @@ __global__ void __launch_bounds__(256) weight_rows_kernel(WeightArgs a)
     const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), lo = lane & 15u, g = lane >> 4, count = (uint32_t)chunk.count;
     for (uint32_t i = threadIdx.x; i < count; i += kThreads) order[i] = a.plan[L.order + (uint32_t)chunk.first + i];
     __syncthreads();
-    const uint32_t col = blockIdx.x * 16u * VEC + VEC * lo, rank0 = blockIdx.z * 16u * RT;
+    const Share mine = share(a.rp / (16u * RT));
+    const uint32_t col = mine.slice * 16u * VEC + VEC * lo, rank0 = mine.half * 16u * RT;
+    if (mine.slice * 16u * VEC >= a.K) return;
     const E* rows = static_cast<const E*>(a.rows.p) + (col < a.K ? col : 0u);
 
     f32x4 acc[RT][VEC] = {};
@@ -890,7 +907,9 @@ __global__ void __launch_bounds__(256, RT == 2 ? 1 : 2) gradient_rows_kernel(Wei
     const uint32_t lane = threadIdx.x & 63u, wave = this_wave(), lo = lane & 15u, g = lane >> 4, count = (uint32_t)chunk.count;
     for (uint32_t i = threadIdx.x; i < count; i += kThreads) order[i] = a.plan[L.order + (uint32_t)chunk.first + i];
     __syncthreads();
-    const uint32_t slice = blockIdx.x, rank0 = blockIdx.z * 16u * RT;
+    const Share part = share(a.rp / (16u * RT));
+    const uint32_t slice = part.slice, rank0 = part.half * 16u * RT;
+    if (slice * 64u * VEC >= a.N) return;
     const uint32_t base = (slice * 4u + wave) * 16u * VEC, col = base + VEC * lo;
     const bool inside = col < a.N;
     const E* rows = static_cast<const E*>(a.rows.p) + (inside ? col : 0u);
@@ -1210,7 +1229,8 @@ int backward(const mi_lora* d, const void* dy, const void* x, const void* A, con
         // dB and d
         float* partials = reinterpret_cast<float*>(ws + b.partials);
         WeightArgs w{plan, rdy, ws + b.pieces[1], tile_down[1], partials, dB, B, P, d->tokens, d->n_adapters, d->rank, b.c.rp, d->K, d->N};
-        dim3 grid(b.slices, (uint32_t)L.max_chunks, b.c.rp / rt);
+        const uint32_t halves = b.c.rp / rt;
+        dim3 grid(shares(b.slices, halves), (uint32_t)L.max_chunks);
         st = for_weights([&](auto r) {
             constexpr int RT = decltype(r)::value;
             if (d->tokens * d->N * sizeof(E) >= kStreamed) hipLaunchKernelGGL((gradient_rows_kernel<E, RT, true>), grid, dim3(kThreads), 0, s, w);
@@ -1231,7 +1251,7 @@ int backward(const mi_lora* d, const void* dy, const void* x, const void* A, con
         w.pieces = ws + b.pieces[0];
         w.down = tile_down[0];
         w.grad = dA;
-        grid.x = (d->K + cols - 1u) / cols;
+        grid.x = shares((d->K + cols - 1u) / cols, halves);
         st = for_weights([&](auto r) {
             hipLaunchKernelGGL((weight_rows_kernel<E, decltype(r)::value>), grid, dim3(kThreads), 0, s, w);
         });
