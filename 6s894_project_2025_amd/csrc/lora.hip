@@ -727,34 +727,45 @@ __device__ __forceinline__ void turn_over(const u32x4 (&in)[4], u32x4 (&out)[4])
         for (int p = 0; p < 4; ++p) out[c][p] = in[p][c];
 }
 
-// One step of the contraction over tokens: acc[j][c] += pieces of 16 ranks (rows) . column VEC lo + c.
+// The pieces of a step's tokens, 16 ranks (rows) each.
 template <class E, int RT>
-__device__ __forceinline__ void weight_step(const WeightArgs& a, uint32_t tile, uint32_t t0, uint32_t rank0, const u32x4 (&in)[Mx<E>::VEC],
-                                            f32x4 (&acc)[RT][Mx<E>::VEC])
+struct Pieces {
+    typename Mx<E>::V of[RT][Mx<E>::PIECES];
+    float down;
+};
+
+template <class E, int RT>
+__device__ __forceinline__ void load_pieces(const WeightArgs& a, uint32_t tile, uint32_t t0, uint32_t rank0, Pieces<E, RT>& w)
+{
+    using X = Mx<E>;
+    const uint32_t lane = threadIdx.x & 63u, lo = lane & 15u, g = lane >> 4;
+    const E* pieces = static_cast<const E*>(a.pieces) + ((uint64_t)tile * a.rp + rank0 + lo) * X::PIECES * 64u + t0 % kTile + X::VEC * g;
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+#pragma unroll
+        for (uint32_t p = 0; p < X::PIECES; ++p) w.of[j][p] = load16<typename X::V>(pieces + (16u * j * X::PIECES + p) * 64u);
+    w.down = X::SCALED ? a.down[tile] : 1.0f;
+}
+
+// One step of the contraction over tokens: acc[j][c] += pieces . column VEC lo + c.
+template <class E, int RT>
+__device__ __forceinline__ void weight_step(const Pieces<E, RT>& w, const u32x4 (&in)[Mx<E>::VEC], f32x4 (&acc)[RT][Mx<E>::VEC])
 {
     using X = Mx<E>;
     using V = typename X::V;
     constexpr uint32_t VEC = X::VEC;
-    const uint32_t lane = threadIdx.x & 63u, lo = lane & 15u, g = lane >> 4;
-    const E* pieces = static_cast<const E*>(a.pieces) + ((uint64_t)tile * a.rp + rank0 + lo) * X::PIECES * 64u + t0 % kTile + VEC * g;
-    V wf[RT][X::PIECES];
-#pragma unroll
-    for (int j = 0; j < RT; ++j)
-#pragma unroll
-        for (uint32_t p = 0; p < X::PIECES; ++p) wf[j][p] = load16<V>(pieces + (16u * j * X::PIECES + p) * 64u);
     u32x4 turned[VEC];
     turn_over(in, turned);
     if constexpr (X::SCALED) {
-        const float down = a.down[tile];
 #pragma unroll
         for (int j = 0; j < RT; ++j)
 #pragma unroll
             for (uint32_t c = 0; c < VEC; ++c) {
                 f32x4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (uint32_t p = 0; p < X::PIECES; ++p) d = X::mma(wf[j][p], __builtin_bit_cast(V, turned[c]), d);
+                for (uint32_t p = 0; p < X::PIECES; ++p) d = X::mma(w.of[j][p], __builtin_bit_cast(V, turned[c]), d);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) acc[j][c][q] = __builtin_fmaf(d[q], down, acc[j][c][q]);
+                for (int q = 0; q < 4; ++q) acc[j][c][q] = __builtin_fmaf(d[q], w.down, acc[j][c][q]);
             }
     } else {
 #pragma unroll
@@ -762,7 +773,7 @@ __device__ __forceinline__ void weight_step(const WeightArgs& a, uint32_t tile, 
 #pragma unroll
             for (uint32_t p = 0; p < X::PIECES; ++p)
 #pragma unroll
-                for (uint32_t c = 0; c < VEC; ++c) acc[j][c] = X::mma(wf[j][p], __builtin_bit_cast(V, turned[c]), acc[j][c]);
+                for (uint32_t c = 0; c < VEC; ++c) acc[j][c] = X::mma(w.of[j][p], __builtin_bit_cast(V, turned[c]), acc[j][c]);
     }
 }
 
@@ -857,13 +868,15 @@ __global__ void __launch_bounds__(256) weight_rows_kernel(WeightArgs a)
     f32x4 acc[RT][VEC] = {};
     for (uint32_t t0 = wave * STEP; t0 < count; t0 += 4u * STEP) {
         u32x4 in[VEC];
+        Pieces<E, RT> w;
+        load_pieces(a, (uint32_t)chunk.tile + t0 / kTile, t0, rank0, w);
 #pragma unroll
         for (uint32_t i = 0; i < VEC; ++i) {
             const uint32_t t = t0 + VEC * g + i;
             in[i] = u32x4{0u, 0u, 0u, 0u};  // tokens behind the chunk: zeros on both sides
             if (t < count) in[i] = load16<u32x4>(rows + (uint64_t)(uint32_t)order[t] * a.rows.stride);
         }
-        weight_step<E, RT>(a, (uint32_t)chunk.tile + t0 / kTile, t0, rank0, in, acc);
+        weight_step<E, RT>(w, in, acc);
     }
 #pragma unroll
     for (uint32_t half = 2; half; half >>= 1) {
@@ -890,6 +903,8 @@ __global__ void __launch_bounds__(256) weight_rows_kernel(WeightArgs a)
 // 16 VEC of the columns and all tokens, STEP at a time with the next requested.  For dB the lanes' registers
 // are turned over as above; for d the same registers go through LDS to become operands along the columns, B
 // stays in registers, and the four wavefronts' sums of a step meet in LDS (two buffers, one barrier a step).
+// A step's pieces are requested before the next step's rows: loads come back in order, and a wait for the
+// pieces must not be one for those rows (8192 tokens, 4096 -> 14336, rank 64: 200 us a call against 220).
 // STREAM: dy is read past the caches (kStreamed).
 template <class E, int RT, bool STREAM>
 __global__ void __launch_bounds__(256, RT == 2 ? 1 : 2) gradient_rows_kernel(WeightArgs a)
@@ -928,6 +943,7 @@ __global__ void __launch_bounds__(256, RT == 2 ? 1 : 2) gradient_rows_kernel(Wei
                 bf[h][j][e] = in ? v : (E)0.0f;
             }
     f32x4 acc[RT][VEC] = {};
+    Pieces<E, RT> w;
     auto request = [&](u32x4 (&in)[VEC], uint32_t t0) __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t i = 0; i < VEC; ++i) {
@@ -936,6 +952,7 @@ __global__ void __launch_bounds__(256, RT == 2 ? 1 : 2) gradient_rows_kernel(Wei
             in[i] = STREAM ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)) : load16<u32x4>(p);
         }
     };
+    auto pieces = [&](uint32_t t0) __attribute__((always_inline)) { load_pieces(a, (uint32_t)chunk.tile + t0 / kTile, t0, rank0, w); };
     auto work = [&](u32x4 (&in)[VEC], uint32_t t0, uint32_t buffer) __attribute__((always_inline)) {
         const u32x4 zero = {0u, 0u, 0u, 0u};
         unsigned char* const mine = own[wave];
@@ -958,7 +975,7 @@ __global__ void __launch_bounds__(256, RT == 2 ? 1 : 2) gradient_rows_kernel(Wei
 #pragma unroll
             for (int j = 0; j < RT; ++j) red[buffer][wave][(s * RT + j) * 64u + lane] = d[j];
         }
-        weight_step<E, RT>(a, (uint32_t)chunk.tile + t0 / kTile, t0, rank0, in, acc);
+        weight_step<E, RT>(w, in, acc);
         __syncthreads();
 #pragma unroll
         for (uint32_t k = 0; k < (UNITS + kThreads - 1u) / kThreads; ++k) {
@@ -975,14 +992,18 @@ __global__ void __launch_bounds__(256, RT == 2 ? 1 : 2) gradient_rows_kernel(Wei
     request(p, 0);
     uint32_t t0 = 0;
     for (; t0 + 2u * STEP < count; t0 += 2u * STEP) {
+        pieces(t0);
         request(q, t0 + STEP);
         work(p, t0, 0);
+        pieces(t0 + STEP);
         request(p, t0 + 2u * STEP);
         work(q, t0 + STEP, 1);
     }
+    pieces(t0);
     if (t0 + STEP < count) {
         request(q, t0 + STEP);
         work(p, t0, 0);
+        pieces(t0 + STEP);
         work(q, t0 + STEP, 1);
     } else {
         work(p, t0, 0);
