@@ -150,6 +150,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     _no_graph("qk_norm_rope", q, k, q_weight, k_weight)
     if inplace and any(n > 1 and s == 0 for t in (q, k) for n, s in zip(t.shape, t.stride())):
         raise RuntimeError("inplace needs heads that do not share memory (an expanded tensor was given)")
+    if inplace and q.data_ptr() == k.data_ptr() and q.numel() and k.numel():
+        raise RuntimeError("inplace needs q and k that do not share memory")
     (qs, qt, qh), (ks, kt, kh) = _readable(q), _readable(k)
     if inplace:
         qo, ko, qot, qoh, kot, koh = qs, ks, qt, qh, kt, kh

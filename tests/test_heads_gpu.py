@@ -487,3 +487,13 @@ def test_lane_layout_covers_every_value_once():
         for bit in range(5):
             other = lane ^ ((2 << bit) - 1)
             assert (lane ^ lane >> 1) ^ (other ^ other >> 1) == 1 << bit
+
+
+@pytest.mark.gpu
+def test_in_place_on_one_memory_is_refused(pkg):
+    q = torch.randn(4, 2, 64, device="cuda")
+    pos, freq = torch.arange(4, device="cuda"), torch.rand(32, device="cuda")
+    with pytest.raises(RuntimeError, match="share memory"):
+        pkg.qk_norm_rope(q, q, None, None, pos, freq, inplace=True)
+    same = pkg.qk_norm_rope(q, q, None, None, pos, freq)
+    assert torch.equal(same[0], same[1])
