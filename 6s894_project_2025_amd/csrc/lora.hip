@@ -19,13 +19,14 @@
 //   weight_rows     dA of a chunk of tokens;  weight_sum adds the weights' parts up
 // All sums are in a fixed order.
 //
-// Bound: HBM.  A rank of 16 is 16 products a value of x and 32 (two pieces) a value of y, far below what
-// the matrix cores do in the time of reading it, so each kernel is one pass over a long matrix, and only the
-// rank-space vectors (rank * 4 bytes a token and part) go between them.  8192 tokens of 8 adapters, 4096 ->
-// 14336, bf16, rank 16: contract_rows 21 us (67 MB), tile_vectors 5, expand_rows 100 (470 MB, 4.7 TB/s: a
-// plain copy of 4 GB reaches 4.7, of 512 MB 5.4).  Backward of 4 adapters: tile_vectors 5 and 5, gradient_rows
-// 50 (235 MB), weight_rows 16, expand_rows 15, weight_sum 6.  Few tokens are bound by their launches
-// (one token: two of 3 us).
+// Bound: HBM.  A rank r is 2r operations a value of x and 4r (two pieces) a value of y, and the matrix cores do
+// hundreds in the time of reading one from memory, so each kernel is one pass over a long matrix, and only
+// rank-space vectors (4r bytes a token and part of the axis) go between them.  8192 tokens, 4096 -> 14336, bf16:
+//   forward, 8 adapters, rank 64: contract_rows 23 us (67 MB in, 15 out), tile_vectors 5, expand_rows 100
+//     (470 MB, 4.8 TB/s with what it reads again; a plain copy of 4 GB reaches 4.7, of 512 MB 5.4)
+//   backward, 4 adapters, rank 16: gradient_rows 48 (219 MB in, 28 out, 5.1 TB/s), weight_rows 13 (67 MB),
+//     expand_rows 15 (67 MB out), weight_sum 6, tile_vectors 5 twice
+// Few tokens are bound by their launches (one token: 3 and 4 us).
 #include <type_traits>
 
 #include "adapter_plan.hpp"

@@ -172,7 +172,7 @@ typedef struct mi_lora {
  *               other overlap with any operand.
  *   shrunk    : NULL, or fp32 [tokens][rank]: receives u (zeros for tokens without an adapter).
  *   workspace : mi_lora_workspace(sizes, 0) bytes.
- * All pointers 16-byte aligned (scales, shrunk: 4).  Two kernels.
+ * All pointers 16-byte aligned (scales, shrunk: 4).  Two kernels, or three where that is faster.
  */
 int mi_lora_add(const void* y, const void* x, const void* A, const void* B, const float* scales,
                 const int32_t* plan, void* out, float* shrunk, void* workspace, const mi_lora* sizes,
