@@ -148,7 +148,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     ``[n, r, K]`` and ``B`` ``[n, N, r]`` the pool of adapters, all in one dtype (fp32, bf16 or fp16), ranks
     that are multiples of 8 up to 128 (a smaller one is padded with zeros), widths that are multiples of
     8.  ``y`` and ``x`` may be column slices of larger matrices.  ``scales`` fp32 ``[n]``.  Sums are fp32, the
-    rank-space vector between the products keeps at least 16 significand bits, and ``out`` is rounded
+    rank-space vector between the products keeps 23 significand bits or more, and ``out`` is rounded
     once.  ``inplace=True`` writes into ``y`` and returns it.  ``return_shrunk=True`` also returns
     ``A[a] @ x[t]``, fp32 ``[tokens, r]``, which :func:`lora_add_backward` takes.
     """

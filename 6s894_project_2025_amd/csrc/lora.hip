@@ -5,10 +5,11 @@
 //   dA  = sum_t d_t x_t^T              dB    = sum_t s g_t u_t^T
 // With r small against K and N all of it is bound by reading x, y (g) and writing out (dx); the matrix
 // cores have time to spare, and the kernels spend some of it on accuracy: u and d stay in 32 bits
-// through being split into two 16-bit pieces, v = hi + lo, which both go through the matrix core
-// (16 significand bits for bf16, 22 for fp16; a single piece would add an error of the size of the
-// output's rounding).  fp16 pieces are taken after a scaling by a power of two, so that neither large
-// nor very small values (gradients) leave the type's range.
+// through being split into 16-bit pieces that all go through the matrix core.  Three bf16 pieces are the
+// fp32 value itself (8 significand bits each).  Two fp16 pieces are within 2^-24 of it (11 bits, 11 of the rest
+// and the rest's sign), what one fp32 rounding adds and less than the sums behind u and d have; they are taken
+// after a scaling by a power of two, so that neither large nor very small values (gradients) leave the
+// type's range.  (Two bf16 pieces, within 2^-18, moved one output in 1500 to a neighbouring bf16 value.)
 //
 // Tokens come grouped by adapter (adapter_plan.hpp), in tiles of up to 64 of one adapter.
 //   contract_rows   P[split][position][r] = sum over a part of the long axis of row . M[a]:  u, and d / s
@@ -19,7 +20,7 @@
 //   weight_rows     dA of a chunk of tokens;  weight_sum adds the weights' parts up
 // All sums are in a fixed order.
 //
-// Bound: HBM.  A rank r is 2r operations a value of x and 4r (two pieces) a value of y, and the matrix cores do
+// Bound: HBM.  A rank r is 2r operations a value of x and 4r or 6r (two or three pieces) a value of y, and the matrix cores do
 // hundreds in the time of reading one from memory, so each kernel is one pass over a long matrix, and only
 // rank-space vectors (4r bytes a token and part of the axis) go between them.  8192 tokens, 4096 -> 14336, bf16:
 //   forward, 8 adapters, rank 64: contract_rows 23 us (67 MB in, 15 out), tile_vectors 5, expand_rows 100
@@ -42,18 +43,21 @@ constexpr uint32_t kThreads = 256;
 // element) is right as long as both operands share it.
 template <class E> struct Mx;
 template <> struct Mx<__bf16> {
-    static constexpr uint32_t VEC = 8, STEP = 32, PIECES = 2;
+    static constexpr int DTYPE = MI_BF16;
+    static constexpr uint32_t VEC = 8, STEP = 32, PIECES = 3;
     static constexpr bool SCALED = false;
     using V = bf16x8;
     static __device__ __forceinline__ f32x4 mma(V a, V b, f32x4 c) { return BF16::mfma32(a, b, c); }
 };
 template <> struct Mx<_Float16> {
+    static constexpr int DTYPE = MI_F16;
     static constexpr uint32_t VEC = 8, STEP = 32, PIECES = 2;
     static constexpr bool SCALED = true;
     using V = f16x8;
     static __device__ __forceinline__ f32x4 mma(V a, V b, f32x4 c) { return F16::mfma32(a, b, c); }
 };
 template <> struct Mx<float> {
+    static constexpr int DTYPE = MI_F32;
     static constexpr uint32_t VEC = 4, STEP = 16, PIECES = 1;
     static constexpr bool SCALED = false;
     using V = f32x4;
@@ -65,14 +69,24 @@ template <> struct Mx<float> {
     }
 };
 
-// hi + lo = v but for the last bits; lo = 0 where hi is not finite, so that an infinity stays one.
-template <class E>
-__device__ __forceinline__ void split(float v, E& hi, E& lo)
+// The sum of the pieces is v (but for the last bits of two); behind a first one that is not finite they are zero, so
+// that an infinity stays one.
+template <class E, uint32_t N>
+__device__ __forceinline__ void split(float v, E (&piece)[N])
 {
-    hi = (E)v;
-    const float rest = v - (float)hi;
-    lo = (E)(__builtin_fabsf((float)hi) < __builtin_inff() ? rest : 0.0f);
+    piece[0] = (E)v;
+    float rest = __builtin_fabsf((float)piece[0]) < __builtin_inff() ? v - (float)piece[0] : 0.0f;
+#pragma unroll
+    for (uint32_t p = 1; p < N; ++p) {
+        piece[p] = (E)rest;
+        rest -= (float)piece[p];  // exact
+    }
 }
+
+// Bytes of a tile's 64 vectors of padded rank rp: as pieces, and as the expansion's operand, where three pieces
+// of 16 ranks take the place of four (Operand::PAIR).
+constexpr uint64_t pieces_bytes(int dtype, uint32_t rp) { return (uint64_t)rp * 64u * (dtype == MI_BF16 ? 6u : 4u); }
+constexpr uint64_t vectors_bytes(int dtype, uint32_t rp) { return dtype == MI_BF16 && rp == 16u ? 8192u : pieces_bytes(dtype, rp); }
 
 // A magnitude for half_scale: what is not finite takes no part.
 __device__ __forceinline__ float finite_magnitude(float v)
@@ -278,17 +292,17 @@ __global__ void __launch_bounds__(256, RT == 8 ? 1 : 2) contract_rows_kernel(Con
 template <class E, int RT>
 struct Operand {
     using X = Mx<E>;
-    static constexpr bool PAIR = X::PIECES == 2 && RT == 1;  // one step: hi in lane groups 0, 1 and lo in 2, 3
-    static constexpr int NF = X::PIECES == 2 ? (RT + 1) / 2 : RT;
-    static constexpr int NP = PAIR ? 1 : (int)X::PIECES;
+    static constexpr bool PAIR = X::PIECES > 1 && RT == 1;  // two pieces a step, one in lane groups 0, 1, one in 2, 3
+    static constexpr int NF = X::PIECES > 1 ? (RT + 1) / 2 : RT;
+    static constexpr int NP = PAIR ? (X::PIECES + 1) / 2 : X::PIECES;
     static constexpr uint32_t COLS = 16u * X::VEC;           // n of a block
     static constexpr uint32_t VECTORS = 4u * NF * NP * 1024u;  // bytes: v of 64 tokens
     static constexpr uint32_t BLOCK = 16u * RT * 256u;         // bytes: M of a block
     // byte offset of piece p of rank r of token t (0 ... 63)
     static __device__ __forceinline__ uint32_t vector_at(uint32_t t, uint32_t r, uint32_t p)
     {
-        const uint32_t f = PAIR ? 0u : r / X::STEP, g = PAIR ? r / 8u + 2u * p : r % X::STEP / X::VEC;
-        return (((t >> 4) * NF + f) * NP + (PAIR ? 0u : p)) * 1024u + (16u * g + (t & 15u)) * 16u + r % X::VEC * (uint32_t)sizeof(E);
+        const uint32_t f = PAIR ? 0u : r / X::STEP, g = PAIR ? r / 8u + 2u * (p & 1u) : r % X::STEP / X::VEC;
+        return (((t >> 4) * NF + f) * NP + (PAIR ? p / 2u : p)) * 1024u + (16u * g + (t & 15u)) * 16u + r % X::VEC * (uint32_t)sizeof(E);
     }
     // byte offset of the 16 bytes that lane (c, g) reads for operand t and fragment f.  Rows n and n + 1 of M
     // come in together and go to operands t and t + 1; the exclusive or spreads them over the banks.
@@ -346,16 +360,17 @@ __device__ __forceinline__ float store_vector(const f32x4 (&v)[RT], uint32_t t, 
         if constexpr (X::PIECES == 1) {
             *reinterpret_cast<f32x4*>(to + O::vector_at(t, r0 + 4u * i, 0)) = v[i];
         } else {
-            E4 hi, low;
+            E4 four[X::PIECES + 1] = {};  // and zeros in an odd pair's other half
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                E h, l;
-                split<E>(v[i][c] * up, h, l);
-                hi[c] = h;
-                low[c] = l;
+                E piece[X::PIECES];
+                split(v[i][c] * up, piece);
+#pragma unroll
+                for (uint32_t p = 0; p < X::PIECES; ++p) four[p][c] = piece[p];
             }
-            *reinterpret_cast<E4*>(to + O::vector_at(t, r0 + 4u * i, 0)) = hi;
-            *reinterpret_cast<E4*>(to + O::vector_at(t, r0 + 4u * i, 1)) = low;
+#pragma unroll
+            for (uint32_t p = 0; p < (O::PAIR ? 2u * O::NP : X::PIECES); ++p)
+                *reinterpret_cast<E4*>(to + O::vector_at(t, r0 + 4u * i, p)) = four[p];
         }
     }
     return down;
@@ -472,14 +487,15 @@ __global__ void __launch_bounds__(256) tile_vectors_kernel(VectorArgs a)
             if constexpr (X::PIECES == 1) {
                 to[0] = v;
             } else {
-                E hi, low;
-                split<E>(v, hi, low);
-                to[0] = hi;
-                to[64] = low;
+                E piece[X::PIECES];
+                split(v, piece);
+#pragma unroll
+                for (uint32_t p = 0; p < X::PIECES; ++p) to[64u * p] = piece[p];
             }
         }
     __syncthreads();
     constexpr uint32_t BYTES = RP * X::PIECES * 64u * sizeof(E);
+    static_assert(BYTES == pieces_bytes(X::DTYPE, RP) && O::VECTORS == vectors_bytes(X::DTYPE, RP), "what the workspace has");
     for (uint32_t i = 16u * threadIdx.x; i < BYTES; i += 16u * kThreads)
         *reinterpret_cast<u32x4*>(static_cast<unsigned char*>(a.pieces) + (uint64_t)blockIdx.x * BYTES + i) =
             *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(turned) + i);
@@ -1121,8 +1137,6 @@ struct Take {  // places in a workspace
     }
 };
 
-uint64_t pieces_bytes(uint32_t rp) { return (uint64_t)rp * 64u * 4u; }  // two of 2 bytes, or one of 4
-
 struct ForwardPlan {
     Cut c;
     bool own;
@@ -1135,7 +1149,7 @@ struct ForwardPlan {
         own = c.few || c.sums() * d->tokens * c.parts <= 1u << 24;
         Take take;
         P = take(c.sums() * d->tokens);
-        vectors = take(own ? 0u : c.max_tiles * pieces_bytes(c.rp));
+        vectors = take(own ? 0u : c.max_tiles * vectors_bytes(d->dtype, c.rp));
         down = take(own ? 0u : c.max_tiles * 64u * 4u);
         bytes = take.end;
     }
@@ -1157,10 +1171,10 @@ struct BackwardPlan {
         Take take;
         P = take((c.sums() > u.sums() ? c.sums() : u.sums()) * d->tokens);  // in turn
         at = take((uint64_t)d->n_adapters * d->rank * d->K * e);
-        vectors = take(c.max_tiles * pieces_bytes(c.rp));
+        vectors = take(c.max_tiles * vectors_bytes(d->dtype, c.rp));
         down = take(c.max_tiles * 64u * 4u);
         for (int i = 0; i < 2; ++i) {
-            pieces[i] = take(c.max_tiles * pieces_bytes(c.rp));
+            pieces[i] = take(c.max_tiles * pieces_bytes(d->dtype, c.rp));
             tile_down[i] = take(c.max_tiles * 4u);
         }
         partials = take(L.max_slots * d->rank * ((uint64_t)d->K + d->N) * 4u);

@@ -165,7 +165,7 @@ typedef struct mi_lora {
  * Low-rank adapters beside a shared projection, each token with its own:
  *     u[t] = A[a] . x[t]      out[t] = y[t] + scales[a] * B[a] . u[t]      a = ids[t] of the plan
  * and out[t] = y[t] for tokens without an adapter.  A [n_adapters][rank][K] and B [n_adapters][N][rank]
- * are dense.  fp32 sums; u is kept to at least 16 significand bits between the products; out is rounded
+ * are dense.  fp32 sums; u is kept to 23 significand bits (fp16; else 24) between the products; out is rounded
  * once.  An adapter of a smaller rank is padded with zeros.  No counterpart in the reference.
  *   scales    : fp32 [n_adapters], or NULL for 1.
  *   out       : may be y with the same stride (in place; other tokens' rows are then not touched); no
