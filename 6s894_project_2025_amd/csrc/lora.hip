@@ -88,6 +88,25 @@ __device__ __forceinline__ void split(float v, E (&piece)[N])
 constexpr uint64_t pieces_bytes(int dtype, uint32_t rp) { return (uint64_t)rp * 64u * (dtype == MI_BF16 ? 6u : 4u); }
 constexpr uint64_t vectors_bytes(int dtype, uint32_t rp) { return dtype == MI_BF16 && rp == 16u ? 8192u : pieces_bytes(dtype, rp); }
 
+// Pieces meet an infinite operand one by one, and the later ones, zero or of the other sign, would make NaN of its
+// infinity.  The first piece alone gives the sign and the class of the whole product, so results that are not
+// finite are replaced by those of the first pieces (computed again: no cost but a sum where all is finite, as
+// a finite result of all pieces has met finite operands only).  An fp16 value below 2^-40 of the largest that it is
+// scaled with has a first piece of zero: that one makes NaN of an infinity.
+template <int N>
+__device__ __forceinline__ bool any_not_finite(const f32x4 (&v)[N])  // the same answer in all lanes
+{
+    f32x4 sum = v[0];  // what is not finite stays so; sums of finite values that overflow only cost time
+#pragma unroll
+    for (int i = 1; i < N; ++i) sum += v[i];
+    return __ballot(!(__builtin_fabsf((sum[0] + sum[1]) + (sum[2] + sum[3])) < __builtin_inff())) != 0;
+}
+__device__ __forceinline__ void take_if_not_finite(f32x4& v, f32x4 first)
+{
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = __builtin_fabsf(v[q]) < __builtin_inff() ? v[q] : first[q];
+}
+
 // A magnitude for half_scale: what is not finite takes no part.
 __device__ __forceinline__ float finite_magnitude(float v)
 {
@@ -610,6 +629,23 @@ __device__ __forceinline__ void expand_blocks(const ExpandArgs& a, const Tile& t
 #pragma unroll
                 for (int p = 0; p < NP; ++p) acc[t] = X::mma(vf[f][p], m, acc[t]);
             }
+        if constexpr (X::PIECES > 1) {
+            if (any_not_finite(acc)) {
+                uint32_t again = cc, group = g;
+                asm volatile("" : "+v"(again), "+v"(group));  // nothing of this is kept in registers on the usual way
+#pragma unroll
+                for (uint32_t t = 0; t < VEC; ++t) {
+                    f32x4 first = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int f = 0; f < NF; ++f) {
+                        V m = *reinterpret_cast<const V*>(from + O::row_at(t, f, again, O::PAIR ? group & 1u : group));
+                        if (O::PAIR && group >= 2u) m = V{};  // what meets the second piece of a pair
+                        first = X::mma(vf[f][0], m, first);
+                    }
+                    take_if_not_finite(acc[t], first);
+                }
+            }
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             V o;
@@ -794,6 +830,46 @@ __device__ __forceinline__ void weight_step(const Pieces<E, RT>& w, const u32x4 
     }
 }
 
+// What infinite rows need (any_not_finite): acc again from the first pieces, for steps t0, t0 + step, ... of the chunk.
+template <class E, int RT>
+__device__ __forceinline__ void mend_infinities(const WeightArgs& a, const E* rows, const int32_t* order, const Chunk& chunk, uint32_t t0, uint32_t step,
+                                                uint32_t rank0, f32x4 (&acc)[RT][Mx<E>::VEC])
+{
+    using X = Mx<E>;
+    using V = typename X::V;
+    constexpr uint32_t VEC = X::VEC;
+    if constexpr (X::PIECES > 1) {
+        const uint32_t count = (uint32_t)chunk.count, lo = threadIdx.x & 15u, g = (threadIdx.x & 63u) >> 4;
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            if (!any_not_finite(acc[j])) continue;
+            f32x4 first[VEC] = {};
+            for (uint32_t t = t0; t < count; t += step) {
+                const uint32_t tile = (uint32_t)chunk.tile + t / kTile;
+                const V w = load16<V>(static_cast<const E*>(a.pieces) +
+                                      ((uint64_t)tile * a.rp + rank0 + 16u * j + lo) * X::PIECES * 64u + t % kTile + VEC * g);
+                const float down = X::SCALED ? a.down[tile] : 1.0f;
+                u32x4 in[VEC], turned[VEC];
+#pragma unroll
+                for (uint32_t i = 0; i < VEC; ++i) {
+                    const uint32_t at = t + VEC * g + i;
+                    in[i] = load16<u32x4>(rows + (uint64_t)(uint32_t)order[at < count ? at : count - 1u] * a.rows.stride);
+                    if (at >= count) in[i] = u32x4{0u, 0u, 0u, 0u};
+                }
+                turn_over(in, turned);
+#pragma unroll
+                for (uint32_t c = 0; c < VEC; ++c) {
+                    const f32x4 d = X::mma(w, __builtin_bit_cast(V, turned[c]), X::SCALED ? f32x4{0.f, 0.f, 0.f, 0.f} : first[c]);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) first[c][q] = X::SCALED ? __builtin_fmaf(d[q], down, first[c][q]) : d[q];
+                }
+            }
+#pragma unroll
+            for (uint32_t c = 0; c < VEC; ++c) take_if_not_finite(acc[j][c], first[c]);
+        }
+    }
+}
+
 // A wavefront's sums: columns col ... col + VEC - 1, ranks rank0 + 16 j + 4 g + q.  To the chunk's partial sums, or
 // rounded to the gradient where the adapter has no other chunk.
 template <class E, int RT, bool DB>
@@ -863,9 +939,10 @@ uint32_t shares(uint32_t slices, uint32_t halves) { return halves == 1u ? slices
 // against 109, though rows are then read once less).  A wavefront takes
 // every fourth step of STEP tokens; a lane reads 16 bytes of VEC consecutive tokens (the 16 lanes of a group
 // read 256 contiguous bytes of a row) and turns them over in registers, one byte permute for two values,
-// so the contraction over tokens needs no LDS.  The wavefronts' sums meet in LDS at the end.
+// so the contraction over tokens needs no LDS.  The wavefronts' sums meet in LDS at the end.  (With three pieces and
+// 32 ranks the compiler takes 192 registers, which leave room for two workgroups on a compute unit; it needs 162.)
 template <class E, int RT>
-__global__ void __launch_bounds__(256) weight_rows_kernel(WeightArgs a)
+__global__ void __launch_bounds__(256, Mx<E>::PIECES == 3 ? 3 : 1) weight_rows_kernel(WeightArgs a)
 {
     using X = Mx<E>;
     constexpr uint32_t VEC = X::VEC, STEP = X::STEP;
@@ -895,6 +972,7 @@ __global__ void __launch_bounds__(256) weight_rows_kernel(WeightArgs a)
         }
         weight_step<E, RT>(w, in, acc);
     }
+    mend_infinities<E, RT>(a, rows, order, chunk, wave * STEP, 4u * STEP, rank0, acc);
 #pragma unroll
     for (uint32_t half = 2; half; half >>= 1) {
         if (wave >= half && wave < 2u * half) {
@@ -1025,6 +1103,7 @@ __global__ void __launch_bounds__(256, RT == 2 ? 1 : 2) gradient_rows_kernel(Wei
     } else {
         work(p, t0, 0);
     }
+    mend_infinities<E, RT>(a, rows, order, chunk, 0, STEP, rank0, acc);
     store_weights<E, RT, true>(a, chunk, rank0, col, acc);
 }
 
