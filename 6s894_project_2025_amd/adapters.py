@@ -4,7 +4,8 @@
 A batch's tokens each name an adapter out of a pool; :func:`adapter_plan` groups them once per batch,
 and every projection of every layer uses the plan.  The projection itself is the caller's, for instance
 :func:`fp8_gemm_rowscale` on rotated activations.  As elsewhere in the package no autograd graph is
-recorded; :func:`lora_add_backward` computes the gradients.
+recorded; :func:`lora_add_backward` computes the gradients.  Differentiable inputs are refused under grad mode, in
+both directions: there are no second derivatives.
 """
 from __future__ import annotations
 
@@ -152,8 +153,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     once.  ``inplace=True`` writes into ``y`` and returns it.  ``return_shrunk=True`` also returns
     ``A[a] @ x[t]``, fp32 ``[tokens, r]``, which :func:`lora_add_backward` takes.
     """
-    T, n, r, K, N = _check(y, x, A, B, plan, scales, "y")
     _no_graph("lora_add", y, x, A, B, scales)
+    T, n, r, K, N = _check(y, x, A, B, plan, scales, "y")
     if inplace and ((T > 1 and y.stride(0) == 0) or y.stride(1) == 0):
         raise RuntimeError("inplace needs rows that do not share memory (an expanded y was given)")
     ys, xs, Ac, Bc = _readable(y), _readable(x), _dense16(A), _dense16(B)
@@ -186,6 +187,7 @@ def lora_add_backward(dy: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: tor
     adapter.  ``dA`` and ``dB`` are in the adapters' dtype, zeros for adapters that no token uses; sums
     over tokens are fp32 in a fixed order.
     """
+    _no_graph("lora_add_backward", dy, x, A, B, scales, shrunk, dx)
     T, n, r, K, N = _check(dy, x, A, B, plan, scales, "dy")
     dev = x.device
     if shrunk is not None and (shrunk.dtype != torch.float32 or tuple(shrunk.shape) != (T, r) or shrunk.device != dev):

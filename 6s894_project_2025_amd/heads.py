@@ -3,7 +3,8 @@ the Hadamard rotation of the head in one pass (``include/mi_hadamard.h``: ``mi_q
 
 Like the other ops of the package these record no autograd graph: the gradients are a function of
 their own, and a differentiable input under an active grad mode is an error rather than a silent
-detach (call them under ``torch.no_grad()`` or inside a ``torch.autograd.Function``).
+detach (call them under ``torch.no_grad()`` or inside a ``torch.autograd.Function``; the gradient
+function has no derivative of its own, so such a Function's backward pass is ``once_differentiable``).
 """
 from __future__ import annotations
 
@@ -146,8 +147,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     positions keep their accuracy; the rest is fp32 with one rounding at the end.
     ``inplace=True`` writes into ``q`` and ``k`` and returns them.
     """
+    _no_graph("qk_norm_rope", q, k, q_weight, k_weight, inv_freq)
     T, D, _, rest = _describe(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, interleaved, hadamard)
-    _no_graph("qk_norm_rope", q, k, q_weight, k_weight)
     if inplace and any(n > 1 and s == 0 for t in (q, k) for n, s in zip(t.shape, t.stride())):
         raise RuntimeError("inplace needs heads that do not share memory (an expanded tensor was given)")
     if inplace and q.data_ptr() == k.data_ptr() and q.numel() and k.numel():
@@ -186,6 +187,7 @@ def qk_norm_rope_backward(q_grad: torch.Tensor, k_grad: torch.Tensor, q: torch.T
     ``None`` has gradient ``None``; the others are in the weights' dtype, summed over all tokens and
     heads in fp32 in a fixed order.
     """
+    _no_graph("qk_norm_rope_backward", q_grad, k_grad, q, k, q_weight, k_weight, inv_freq)
     T, D, wdt, rest = _describe(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, interleaved, hadamard)
     for g, t, n in ((q_grad, q, "q_grad"), (k_grad, k, "k_grad")):
         if g.shape != t.shape or g.dtype is not t.dtype:

@@ -58,7 +58,11 @@ def _dense16(t: torch.Tensor) -> torch.Tensor:
 
 
 def _no_graph(name: str, *tensors) -> None:
+    """Refuses differentiable inputs, which an op that records no graph would detach."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        if name.endswith("_backward"):
+            raise RuntimeError(f"{name} records no autograd graph, so there are no second derivatives: call it under "
+                               "torch.no_grad(), and not from a backward pass with create_graph=True")
         raise RuntimeError(f"{name} records no autograd graph: call it under torch.no_grad() or inside a "
                            f"torch.autograd.Function, and {name}_backward for the gradients")
 
