@@ -11,6 +11,7 @@ import contextlib
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -58,13 +59,19 @@ def _dense16(t: torch.Tensor) -> torch.Tensor:
 
 
 def _no_graph(name: str, *tensors) -> None:
-    """Refuses differentiable inputs, which an op that records no graph would detach."""
+    """Refuses differentiable inputs, which an op that records no graph would detach: of reverse mode under grad
+    mode, and dual tensors of forward mode."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         if name.endswith("_backward"):
             raise RuntimeError(f"{name} records no autograd graph, so there are no second derivatives: call it under "
                                "torch.no_grad(), and not from a backward pass with create_graph=True")
         raise RuntimeError(f"{name} records no autograd graph: call it under torch.no_grad() or inside a "
                            f"torch.autograd.Function, and {name}_backward for the gradients")
+    # a level is open inside forward_ad.dual_level() only; an autograd.Function's forward sees dual tensors with
+    # forward mode off
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise RuntimeError(f"{name} records no autograd graph: forward-mode tangents would be lost")
 
 
 def hadamard_transform(x: torch.Tensor, scale: float | None = None, *, inplace: bool = False

@@ -1,8 +1,9 @@
 """The adapter and head operators record no autograd graph, and refuse inputs whose derivatives would be lost: all four
-functions, each differentiable operand.  The refusal comes before the device is
+functions, each differentiable operand, reverse and forward mode.  The refusal comes before the device is
 looked at, so it is tested on the CPU; on the GPU inside autograd functions."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from test_adapters_gpu import _Plan, make, on_gpu
@@ -44,6 +45,20 @@ def test_differentiable_operands_are_refused(pkg, call, name):
         run(pkg, **o)
     with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):  # the next check
         run(pkg, **o)
+
+
+@pytest.mark.parametrize("call,name", OPERANDS)
+def test_dual_operands_are_refused(pkg, call, name):
+    run, operands = CALLS[call]
+    o = operands()
+    with forward_ad.dual_level():
+        o[name] = forward_ad.make_dual(o[name], torch.ones_like(o[name]))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(RuntimeError, match=f"{call} records no autograd graph: forward-mode"):
+                run(pkg, **o)
+        o[name] = forward_ad.unpack_dual(o[name]).primal
+        with pytest.raises(RuntimeError, match="GPU"):
+            run(pkg, **o)
 
 
 def functions(pkg, decorate):
