@@ -16,7 +16,7 @@ import struct
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _dense16, _no_graph, _on_device_of, _require_cuda, _stream
+from .ops import _DTYPE_CODE, _dense16, _no_graph, _on_device_of, _require_cuda, _stream, _written
 
 MAX_ADAPTERS, MAX_TOKENS, MAX_RANK, MAX_WIDTH = 1024, 1 << 24, 128, 1 << 22
 _LORA = struct.Struct("<4Q4Ii4x")  # mi_lora
@@ -173,6 +173,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     if inplace:
         if ys is not y:
             y.copy_(ys)
+        else:
+            _written(y)
         out = y
     return (out, shrunk) if return_shrunk else out
 
@@ -214,5 +216,7 @@ def lora_add_backward(dy: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: tor
     if dx is not None:
         if into is not dx:
             dx.copy_(into)
+        else:
+            _written(dx)
         into = dx
     return into, dA, dB

@@ -13,7 +13,7 @@ import struct
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _dense16, _is_pow2, _no_graph, _on_device_of, _require_cuda, _stream
+from .ops import _DTYPE_CODE, _dense16, _is_pow2, _no_graph, _on_device_of, _require_cuda, _stream, _written
 
 _NEIGHBOURS, _HADAMARD = 1, 2
 _HEADS = struct.Struct("<Q6Q6Q4I" "I4I" "iiIII" "f4x")  # mi_heads
@@ -170,10 +170,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
                                      ko.data_ptr(), _HEADS.pack(T, qt, kt, qot, kot, 0, 0, qh, kh, qoh, koh, 0, 0, *rest), _stream(q))
         _lib.check(st, "qk_norm_rope")
     if inplace:
-        if qs is not q:
-            q.copy_(qs)
-        if ks is not k:
-            k.copy_(ks)
+        for given, written in ((q, qs), (k, ks)):
+            if written is not given:
+                given.copy_(written)
+            else:
+                _written(given)
         return q, k
     return qo, ko
 

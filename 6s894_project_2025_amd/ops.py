@@ -74,6 +74,13 @@ def _no_graph(name: str, *tensors) -> None:
             raise RuntimeError(f"{name} records no autograd graph: forward-mode tangents would be lost")
 
 
+def _written(t: torch.Tensor) -> None:
+    """Tells autograd that a kernel has written into ``t``: a saved ``t`` is then refused by a backward pass, as
+    after torch's own in-place functions.  (Inference tensors have no version.)"""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def hadamard_transform(x: torch.Tensor, scale: float | None = None, *, inplace: bool = False
                        ) -> torch.Tensor:
     """Walsh-Hadamard transform over the last dimension: ``y = scale * x @ H_n``.
