@@ -16,7 +16,7 @@ import struct
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _dense16, _no_graph, _on_device_of, _require_cuda, _stream, _written
+from .ops import _DTYPE_CODE, _apart, _dense16, _no_graph, _on_device_of, _require_cuda, _stream, _written
 
 MAX_ADAPTERS, MAX_TOKENS, MAX_RANK, MAX_WIDTH = 1024, 1 << 24, 128, 1 << 22
 _LORA = struct.Struct("<4Q4Ii4x")  # mi_lora
@@ -84,6 +84,11 @@ def adapter_plan(ids: torch.Tensor, n_adapters: int) -> AdapterPlan:
 def _row_stride(t: torch.Tensor) -> int:
     """Row stride in elements; one row's stride means nothing."""
     return t.stride(0) if t.size(0) > 1 else 0
+
+
+def _rows_apart(t: torch.Tensor) -> bool:
+    row, column = t.stride()
+    return column == 1 and row >= t.size(1) or _apart(t)
 
 
 def _ptr(t):
@@ -155,8 +160,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     """
     _no_graph("lora_add", y, x, A, B, scales)
     T, n, r, K, N = _check(y, x, A, B, plan, scales, "y")
-    if inplace and ((T > 1 and y.stride(0) == 0) or y.stride(1) == 0):
-        raise RuntimeError("inplace needs rows that do not share memory (an expanded y was given)")
+    if inplace and not _rows_apart(y):
+        raise RuntimeError("inplace needs a y whose elements do not share memory")
     ys, xs, Ac, Bc = _readable(y), _readable(x), _dense16(A), _dense16(B)
     out = ys if inplace else torch.empty_like(ys, memory_format=torch.contiguous_format)
     shrunk = torch.empty((T, r), dtype=torch.float32, device=x.device) if return_shrunk else None
@@ -185,7 +190,7 @@ def lora_add_backward(dy: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: tor
     """Gradients of :func:`lora_add`: ``(dx, dA, dB)`` from ``dy``, the gradient of ``out`` (the gradient of ``y``
     is ``dy`` itself).  ``shrunk`` is what the forward call returned with ``return_shrunk``; without it
     ``A[a] @ x[t]`` is computed again.  With ``dx`` given (the shared projection's own gradient) the
-    adapters' part is added to it in place (it may be ``x`` itself); without, a new tensor with zeros for tokens without an
+    adapters' part is added to it in place; without, a new tensor with zeros for tokens without an
     adapter.  ``dA`` and ``dB`` are in the adapters' dtype, zeros for adapters that no token uses; sums
     over tokens are fp32 in a fixed order.
     """
@@ -197,8 +202,8 @@ def lora_add_backward(dy: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: tor
     if dx is not None:
         if dx.shape != x.shape or dx.dtype != x.dtype or dx.device != dev:
             raise RuntimeError(f"dx must be like x: {tuple(x.shape)} {x.dtype} on {dev}")
-        if (T > 1 and dx.stride(0) == 0) or dx.stride(1) == 0:
-            raise RuntimeError("dx needs rows that do not share memory (an expanded tensor was given)")
+        if not _rows_apart(dx):
+            raise RuntimeError("dx needs elements that do not share memory")
     gs, xs, Ac, Bc = _readable(dy), _readable(x), _dense16(A), _dense16(B)
     into = torch.empty_like(xs, memory_format=torch.contiguous_format) if dx is None else _readable(dx)
     dA, dB = torch.empty_like(Ac), torch.empty_like(Bc)

@@ -13,7 +13,7 @@ import struct
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _dense16, _is_pow2, _no_graph, _on_device_of, _require_cuda, _stream, _written
+from .ops import _DTYPE_CODE, _apart, _dense16, _is_pow2, _no_graph, _on_device_of, _require_cuda, _stream, _written
 
 _NEIGHBOURS, _HADAMARD = 1, 2
 _HEADS = struct.Struct("<Q6Q6Q4I" "I4I" "iiIII" "f4x")  # mi_heads
@@ -149,10 +149,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     """
     _no_graph("qk_norm_rope", q, k, q_weight, k_weight, inv_freq)
     T, D, _, rest = _describe(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, interleaved, hadamard)
-    if inplace and any(n > 1 and s == 0 for t in (q, k) for n, s in zip(t.shape, t.stride())):
-        raise RuntimeError("inplace needs heads that do not share memory (an expanded tensor was given)")
-    if inplace and q.data_ptr() == k.data_ptr() and q.numel() and k.numel():
-        raise RuntimeError("inplace needs q and k that do not share memory")
+    if inplace and not _apart(q, k):
+        raise RuntimeError("inplace needs q and k whose elements do not share memory")
     (qs, qt, qh), (ks, kt, kh) = _readable(q), _readable(k)
     if inplace:
         qo, ko, qot, qoh, kot, koh = qs, ks, qt, qh, kt, kh

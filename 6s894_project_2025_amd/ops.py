@@ -81,6 +81,55 @@ def _written(t: torch.Tensor) -> None:
         torch.autograd.graph.increment_version(t)
 
 
+def _span(shape, strides) -> tuple[int, bool]:
+    """Elements from a tensor's first to behind its last, and whether the strides alone show that no two of them
+    share memory: each axis steps over all that the shorter ones cover."""
+    extent, clear = 1, True
+    for stride, size in sorted(zip(strides, shape)):
+        if size > 1:
+            if stride < extent:
+                clear = False
+            extent += stride * (size - 1)
+        elif size == 0:
+            return 0, True
+    return extent, clear
+
+
+def _apart(t: torch.Tensor, other: torch.Tensor | None = None) -> bool:
+    """Whether no two elements of ``t`` (and of ``other``, of its dtype) share memory."""
+    shape, strides = t.shape, t.stride()
+    extent, clear = _span(shape, strides)
+    if other is None:
+        return clear or _apart_one_by_one(t)
+    other_shape, other_strides = other.shape, other.stride()
+    e, c = _span(other_shape, other_strides)
+    if clear and c:
+        size, gap = t.element_size(), other.data_ptr() - t.data_ptr()
+        if not extent or not e or gap >= extent * size or -gap >= e * size:
+            return True
+        # slices of the rows of one matrix: the first axis steps over what each covers of a row
+        row = strides[0]
+        if row and row == other_strides[0] and gap % size == 0:
+            at = gap // size % row
+            if extent - row * (shape[0] - 1) <= at and at + e - row * (other_shape[0] - 1) <= row:
+                return True
+    return _apart_one_by_one(t, other)
+
+
+def _apart_one_by_one(*tensors: torch.Tensor) -> bool:
+    """The same by the places of all elements, or of all rows where these are contiguous."""
+    rows = all(t.stride(-1) == 1 or t.size(-1) == 1 for t in tensors)
+    places, lengths = [], []
+    for t in tensors:
+        at = torch.full((1,), t.data_ptr(), dtype=torch.int64)
+        for stride, n in zip(t.stride()[:-1] if rows else t.stride(), t.shape):
+            at = (at[:, None] + torch.arange(n) * (stride * t.element_size())).flatten()
+        places.append(at)
+        lengths.append(torch.full_like(at, t.element_size() * (t.size(-1) if rows else 1)))
+    place, order = torch.sort(torch.cat(places))
+    return bool((place[:-1] + torch.cat(lengths)[order][:-1] <= place[1:]).all())
+
+
 def hadamard_transform(x: torch.Tensor, scale: float | None = None, *, inplace: bool = False
                        ) -> torch.Tensor:
     """Walsh-Hadamard transform over the last dimension: ``y = scale * x @ H_n``.
