@@ -254,26 +254,73 @@ def check_m0_is_the_transfers_alone(asm_text: str, where: str) -> int:
     return writes
 
 
+_EXEC_NARROWED = re.compile(r"s_(?!or_)\w*saveexec_b64|s_(and|andn2|xor|nand|nor|xnor)_b64 exec,|s_mov_b64 exec, (?!-1$)|v_cmpx_")
+_EXEC_RESTORED = re.compile(r"s_or_b64 exec,|s_or_saveexec_b64")
+
+
 def check_no_masked_mfma(asm_text: str, where: str) -> int:
     """Matrix-core instructions ignore the lane mask.  Where the compiler takes a condition to differ
-    between lanes it may save and narrow EXEC and run the conditional code without a branch around it;
-    an MFMA in there then executes for wavefronts that should have skipped it, and corrupts their
-    accumulators.  Raises if an MFMA stands behind such a narrowing with neither a branch nor a label nor
-    the restoring of EXEC in between; returns the number of MFMAs checked."""
-    checked, name, masked = 0, None, None
-    for line in asm_text.splitlines():
-        text = line.split(";")[0].strip()
-        label = _ANY_LABEL.match(text)
-        if label:
-            name, masked = (label.group(1), None) if not label.group(1).startswith(".") else (name, None)
-        elif text.startswith("s_and_saveexec"):
-            masked = text
-        elif text.startswith(("s_cbranch", "s_branch", "s_or_b64 exec", "s_mov_b64 exec")):
-            masked = None
-        elif text.startswith("v_mfma"):
-            checked += 1
-            if masked:
-                raise RuntimeError(f"{where}: {name}: `{text}` executes whatever `{masked}` leaves of the wavefront")
+    between lanes it narrows EXEC and may run the conditional code, or its other side, without a branch around
+    it; an MFMA in there then executes for wavefronts that should have skipped it, and corrupts their
+    accumulators.  Raises if, on any path the branches allow, an MFMA stands behind an instruction that may have
+    left EXEC empty, with neither a branch that is taken for an empty EXEC (s_cbranch_execz, the way on from
+    s_cbranch_execnz) nor the restoring of EXEC in between; returns the number of MFMAs checked.  What a branch on
+    EXEC lets pass has some lanes: it is for the source to see to it that these are all or none."""
+    checked = 0
+    lines = asm_text.splitlines()
+    i = 0
+    while i < len(lines):
+        label = _LABEL.match(lines[i])
+        if not label:
+            i += 1
+            continue
+        name = label.group(1)
+        ins, labels = [], {}
+        i += 1
+        while i < len(lines) and not _LABEL.match(lines[i]):
+            text = lines[i].split(";")[0].strip()
+            local = _ANY_LABEL.match(text)
+            if local:
+                labels[local.group(1)] = len(ins)
+            elif text and not text.startswith("."):
+                ins.append(text)
+            i += 1
+        checked += sum(t.startswith("v_mfma") for t in ins)
+        seen = set()
+        todo = [(0, ())]  # position; what may have emptied EXEC since: instructions and where they saved it
+        while todo:
+            k, masked = todo.pop()
+            while k < len(ins) and (k, masked) not in seen:
+                seen.add((k, masked))
+                t = ins[k]
+                op = t.split()[0]
+                k += 1
+                if op == "s_endpgm":
+                    break
+                if op == "s_branch":
+                    k = labels.get(t.split()[1], len(ins))
+                elif op.startswith("s_cbranch"):
+                    to = labels.get(t.split()[1], len(ins))
+                    if op == "s_cbranch_execz":  # not taken where nothing has narrowed EXEC
+                        todo += [(to, masked)] if masked else []
+                        masked = ()
+                    elif op == "s_cbranch_execnz":
+                        todo.append((to, ()))
+                        k = k if masked else len(ins)
+                    else:
+                        todo.append((to, masked))
+                elif op == "s_mov_b64" and t.endswith("exec, -1"):
+                    masked = ()
+                elif _EXEC_RESTORED.match(t):  # from a register: to what was when it was saved
+                    saved = t.split()[-1]
+                    depth = [n for n, (_, where_to) in enumerate(masked) if where_to == saved]
+                    masked = masked[:depth[0] if depth else -1]
+                elif _EXEC_NARROWED.match(t):
+                    saved = t.split()[1].rstrip(",") if "saveexec" in op else None
+                    if (t, saved) not in masked:
+                        masked += ((t, saved),)
+                elif masked and op.startswith("v_mfma"):
+                    raise RuntimeError(f"{where}: {name}: `{t}` executes whatever `{masked[-1][0]}` leaves of the wavefront")
     return checked
 
 
