@@ -10,7 +10,8 @@ namespace adapters {
 constexpr uint32_t kTile = 64;        // tokens of one adapter that a workgroup takes together
 constexpr uint32_t kMaxChunk = 512;
 constexpr uint32_t kMaxAdapters = 1024;
-// A grid has at most 65535 workgroups along its second axis, where chunks and parts of K or N are.
+// A grid has at most 65535 workgroups along its second axis, where chunks are: 2^24 tokens and 1024 adapters give
+// 33793.  Along the first are tiles times parts of K or N, below 2^32 threads; columns are counted in 32 bits.
 constexpr uint64_t kMaxTokens = 1u << 24;
 constexpr uint32_t kMaxWidth = 1u << 22;
 
@@ -33,9 +34,9 @@ struct PlanLayout {
         max_tiles = tokens / kTile + used;
         chunk = tokens < 4096u ? 128u : tokens < 8192u ? 256u : 512u;
         max_chunks = tokens / chunk + used;
-        // only adapters with more than `chunk` tokens have slots: at most tokens / chunk of them, and
-        // ceil(c / chunk) <= 2 c / chunk for each
-        max_slots = 2u * (tokens / chunk);
+        // only adapters with more than `chunk` tokens have slots: at most n and at most tokens / chunk of them, each
+        // with ceil(c / chunk) <= floor(c / chunk) + 1, and the floors add up to at most tokens / chunk
+        max_slots = tokens / chunk + (n < tokens / chunk ? n : tokens / chunk);
         chunks = 4u * max_tiles;
         counts = chunks + 8u * max_chunks;  // {tiles, chunks}
         slot_start = counts + 2u;           // [n]

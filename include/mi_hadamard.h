@@ -192,7 +192,14 @@ int mi_lora_add(const void* y, const void* x, const void* A, const void* B, cons
 int mi_lora_add_backward(const void* dy, const void* x, const void* A, const void* B, const float* scales,
                          const int32_t* plan, const float* shrunk, const void* dx_in, void* dx, void* dA,
                          void* dB, void* workspace, const mi_lora* sizes, void* stream);
-/* Bytes of workspace, 16-byte aligned; 0 for sizes that the calls refuse. */
+/*
+ * Bytes of workspace, 16-byte aligned; 0 for sizes that the calls refuse.  With R the rank padded to 16, 32, 64 or
+ * 128: the forward pass takes 4 R tokens for each part of K, eight of them (more with few tokens), and 6 R tokens
+ * for vectors.  The backward pass grows with the batch in three ways: 4 R tokens N / 512 (fp32: N / 256) for parts of d, 18 R tokens
+ * for vectors, and, from 8192 tokens on, 4 rank (K + N) bytes for each 512 tokens and for each adapter with more
+ * than 512 (smaller batches: 256 and 128); and it holds a transposed copy of all of A.  65536 tokens of 8
+ * adapters of rank 64, 4096 -> 14336, bf16: 1.2 GB.
+ */
 uint64_t mi_lora_workspace(const mi_lora* sizes, int backward);
 
 /*
