@@ -1222,10 +1222,13 @@ struct ForwardPlan {
     uint64_t P, vectors, down, bytes;
     explicit ForwardPlan(const mi_lora* d) : c(d, d->K, d->N)
     {
-        // a launch less where adding up P again in every workgroup moves no more than 16 MB: 64 tokens of 48
-        // adapters, 4096 -> 14336, rank 16 (4 MB) 18.3 us a call against 22.5, of which the GPU works 16.0 and
-        // 14.6; 512 tokens of 64 adapters, rank 64 (58 MB) 62 against 51
-        own = c.few || c.sums() * d->tokens * c.parts <= 1u << 24;
+        // A launch less where adding up P again in every workgroup moves no more than 16 MB of sums, and where the
+        // workgroups, which read 64 tokens' whatever their tile has, read no more than 192 MB from the caches.  4096 ->
+        // 14336, us a call (in a graph): 64 tokens of 48 adapters, rank 16 (176 MB read) 18.5 (16.4) against 21.2
+        // (15.7), rank 32 (350) 22.8 (23.4) against 21.2 (19.1), rank 64 (700) 50 (50) against 32 (32); 256 tokens
+        // of 64, rank 16 (120) 20.7 (20.9) against 21.2 (19.9).  4096 -> 4096, rank 64 (200) 23.8 (24.5) against 21.5
+        // (21.6).  512 tokens of 64 adapters, 4096 -> 14336, rank 64 (58 MB moved): 62 against 51.
+        own = c.few || (c.sums() * c.parts * d->tokens <= 16u << 20 && c.sums() * c.parts * c.max_tiles * 64u <= 192u << 20);
         Take take;
         P = take(c.sums() * d->tokens);
         vectors = take(own ? 0u : c.max_tiles * vectors_bytes(d->dtype, c.rp));

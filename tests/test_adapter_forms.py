@@ -24,6 +24,8 @@ def cases():
         for r in (8, 16, 24, 40, 64, 72, 128):
             yield 333, 3, r, 9 * block + 24, 9 * block + 8, dtype, "mixed"        # 16 tokens a workgroup
             yield 1300, 3, r, 3 * block + 40, 5 * block + 24, dtype, "mixed"      # own sums
+            if r == 128:  # few tokens of many adapters: too much to add up again in every workgroup
+                yield 70, 60, r, 19 * block + 8, 60 * block + 8, dtype, "mixed"
             yield 4390, 7, r, 19 * block + 8, 17 * block + 40, dtype, "runs" if r == 40 else "mixed"  # vectors made once
 
 
@@ -39,7 +41,8 @@ def test_cases_reach_every_form():
         c = Cut(T, n, r, K, N, CODE[dtype])
         if form(T, n, r, K, N, dtype) != "own":
             assert c.splits > 1 and c.parts > 1
-    # on both sides of the border between the last two, at one size and type
+    # on both sides of the borders between the last two
+    assert [form(70, 60, r, 19 * 128 + 8, 60 * 128 + 8, "bf16") for r in (64, 72)] == ["own", "vectors"]
     near = [form(4390, 7, 8, 19 * 128 + 8, N, "bf16") for N in range(128, 4096, 128)]
     assert near[0] == "own" and near[-1] == "vectors" and near == sorted(near)
 

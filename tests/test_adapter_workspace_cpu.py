@@ -41,7 +41,7 @@ class Cut:
         self.splits = cut(self.tiles, -(-K // block), 4 if self.few else 2, 1024)
         self.parts = cut(self.tiles, -(-N // block), 4 if self.few else 2, 1024 if self.few else 8192)
         self.sums = self.splits * padded(r) * 4
-        self.own = self.few or self.sums * T * self.parts <= 1 << 24
+        self.own = self.few or (self.sums * self.parts * T <= 16 << 20 and self.sums * self.parts * self.tiles * 64 <= 192 << 20)
 
 
 def whole(*sizes):
