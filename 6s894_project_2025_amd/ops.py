@@ -107,13 +107,25 @@ def _apart(t: torch.Tensor, other: torch.Tensor | None = None) -> bool:
         size, gap = t.element_size(), other.data_ptr() - t.data_ptr()
         if not extent or not e or gap >= extent * size or -gap >= e * size:
             return True
-        # slices of the rows of one matrix: the first axis steps over what each covers of a row
-        row = strides[0]
-        if row and row == other_strides[0] and gap % size == 0:
-            at = gap // size % row
-            if extent - row * (shape[0] - 1) <= at and at + e - row * (other_shape[0] - 1) <= row:
-                return True
+        # slices of the rows of one matrix, or heads in turn: modulo a stride each covers a range of its own
+        if gap % size == 0:
+            for step in {*strides, *other_strides}:
+                if step > 1:
+                    at = gap // size % step
+                    first, second = _residues(shape, strides, step), _residues(other_shape, other_strides, step)
+                    if first <= at and at + second <= step:
+                        return True
     return _apart_one_by_one(t, other)
+
+
+def _residues(shape, strides, step: int) -> int:
+    """How many residues modulo ``step`` a tensor's elements have from its first one's on: those of the axes with
+    smaller strides, or all where a larger one is no multiple."""
+    extent = 1
+    for stride, size in zip(strides, shape):
+        if size > 1 and stride % step:
+            extent += step if stride > step else stride * (size - 1)
+    return extent
 
 
 def _apart_one_by_one(*tensors: torch.Tensor) -> bool:

@@ -89,3 +89,38 @@ def test_operators_refuse_shared_memory_in_place(pkg):
         with pytest.raises(RuntimeError, match="share memory"):
             pkg.lora_add_backward(bf(T, N), x, A, B, plan, dx=dx)
         pkg.lora_add(y, x, A, B, plan)
+
+
+def test_layouts_of_use_are_told_from_their_strides(pkg, monkeypatch):
+    """The comparison of all rows takes 40 ms for 8192 tokens of 64 heads: no usual layout comes to it."""
+    ops = importlib.import_module(pkg.__name__ + ".ops")
+    monkeypatch.setattr(ops, "_apart_one_by_one", lambda *tensors: pytest.fail("compared one by one"))
+    T, H, D = 8192, 32, 128
+    packed = torch.empty(T, (H + 16) * D, device="meta")
+    per_head = torch.empty(T, H, 3, D, device="meta")
+    per_group = torch.empty(T, 8, 6, D, device="meta")
+    heads_first = torch.empty(H + 16, T, D, device="meta")
+    pairs = torch.empty(T, H, D, 2, device="meta")
+    for q, k in ((packed[:, :H * D].unflatten(1, (H, D)), packed[:, H * D:(H + 8) * D].unflatten(1, (8, D))),
+                 (packed[:, 16 * D:].unflatten(1, (H, D)), packed[:, :8 * D].unflatten(1, (8, D))),
+                 (per_head[:, :, 0], per_head[:, :, 1]), (per_head[:, :, 2], per_head[:, :, 0]),
+                 (per_group[:, :, 3], per_group[:, :, 4]),
+                 (heads_first[:H].transpose(0, 1), heads_first[H:H + 8].transpose(0, 1)),
+                 (pairs[..., 0], pairs[..., 1]), (packed[:1, :H * D].unflatten(1, (H, D)), packed[1:2, :D].unflatten(1, (1, D)))):
+        assert at_addresses(ops._apart, q, k)
+        assert ops._apart(q) and ops._apart(k)
+
+
+def at_addresses(f, *tensors):
+    """A call on tensors without memory, which have offsets but no addresses."""
+    class At:
+        def __init__(self, t):
+            self.t, self.shape = t, t.shape
+
+        def data_ptr(self):
+            return (1 << 20) + self.t.storage_offset() * self.t.element_size()
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+    return f(*(At(t) for t in tensors))
