@@ -1179,9 +1179,9 @@ int check(const mi_lora* d)
 
 // How a batch is cut.  With at most 16 tiles workgroups take 16 tokens instead of 64, their wavefronts take
 // different parts of the adapter, which is then most of what there is to read, and the expansion adds up the
-// parts of P itself, a launch less (rank 16, 4096 -> 4096, one token 6.7 us against 8.5, 64 tokens of four
-// adapters 7.1 against 9.5).  With more tiles the four times as many workgroups cost more than that (64
-// tokens of 48 adapters, 4096 -> 14336: 17 us against 13.6).
+// parts of P itself, a launch less (rank 16, 4096 -> 4096, in a graph: one token 7.1 us against 8.5, 64 tokens of
+// four adapters 7.1 against 9.5).  With more tiles the four times as many workgroups cost more than that (64
+// tokens of 48 adapters, 4096 -> 14336: 19.8 us against 16.4).
 struct Cut {
     bool few;
     uint32_t rp, splits, parts;
@@ -1202,8 +1202,10 @@ struct Cut {
     uint64_t sums() const { return (uint64_t)splits * rp * 4u; }  // bytes of P per token
 };
 
-// From so many bytes of dy on it is read past the caches, a quarter of the last of which it would fill (rank 16:
-// 235 MB 97 us a call against 102, 67 MB 69 against 74; but 59 MB 48.4 against 45.9, 29 MB 38.5 against 35).
+// From so many bytes of dy on it is read past the caches, a quarter of the last of which it would fill.  Rank 16:
+// 235 MB 92.6 us a call against 100.1, 67 MB 69 against 74; but 59 MB 48.4 against 45.9, 29 MB 38.5 against 35.
+// Several halves of the ranks, which read the same rows soon after each other, gain less but lose nothing by it:
+// 235 MB at rank 64 221 against 224, in fp16 207 against 210, at rank 128 416 against 419.
 constexpr uint64_t kStreamed = 64u << 20;
 
 struct Take {  // places in a workspace
