@@ -23,10 +23,12 @@
 // Bound: HBM.  A rank r is 2r operations a value of x and 4r or 6r (two or three pieces) a value of y, and the matrix cores do
 // hundreds in the time of reading one from memory, so each kernel is one pass over a long matrix, and only
 // rank-space vectors (4r bytes a token and part of the axis) go between them.  8192 tokens, 4096 -> 14336, bf16:
-//   forward, 8 adapters, rank 64: contract_rows 23 us (67 MB in, 15 out), tile_vectors 5, expand_rows 100
+//   forward, 8 adapters, rank 64: contract_rows 23 us (67 MB in, 15 out), tile_vectors 6, expand_rows 104
 //     (470 MB, 4.8 TB/s with what it reads again; a plain copy of 4 GB reaches 4.7, of 512 MB 5.4)
-//   backward, 4 adapters, rank 16: gradient_rows 48 (219 MB in, 28 out, 5.1 TB/s), weight_rows 13 (67 MB),
-//     expand_rows 15 (67 MB out), weight_sum 6, tile_vectors 5 twice
+//   backward, 4 adapters, rank 16: gradient_rows 50 (206 MB in, 26 out, 4.6 TB/s), weight_rows 14 (67 MB),
+//     expand_rows 15 (67 MB out), weight_sum 5, tile_vectors 5 twice
+//   the same of rank 64: gradient_rows 149 (235 MB in, 107 out), weight_rows 35, expand_rows 20, weight_sum 14,
+//     tile_vectors 5 and 12: no longer the bytes, but what a step waits for with one wavefront per SIMD
 // Few tokens are bound by their launches (one token: 3 and 4 us).
 #include <type_traits>
 
@@ -935,8 +937,8 @@ __device__ __forceinline__ Share share(uint32_t halves)
 uint32_t shares(uint32_t slices, uint32_t halves) { return halves == 1u ? slices : (slices + 7u) / 8u * 8u * halves; }
 
 // dA.  Workgroup: a chunk of tokens of one adapter, 16 VEC columns of x, RT * 16 ranks (32 at most: with 64 the
-// registers leave one wavefront per SIMD: a backward pass of 8192 tokens, 4096 -> 4096, rank 64 took 130 us
-// against 109, though rows are then read once less).  A wavefront takes
+// registers leave one wavefront per SIMD: a backward pass of 8192 tokens, 4096 -> 4096, rank 64, two pieces, took
+// 130 us against 109, though rows are then read once less).  A wavefront takes
 // every fourth step of STEP tokens; a lane reads 16 bytes of VEC consecutive tokens (the 16 lanes of a group
 // read 256 contiguous bytes of a row) and turns them over in registers, one byte permute for two values,
 // so the contraction over tokens needs no LDS.  The wavefronts' sums meet in LDS at the end.  (With three pieces and
@@ -999,7 +1001,7 @@ __global__ void __launch_bounds__(256, Mx<E>::PIECES == 3 ? 3 : 1) weight_rows_k
 // are turned over as above; for d the same registers go through LDS to become operands along the columns, B
 // stays in registers, and the four wavefronts' sums of a step meet in LDS (two buffers, one barrier a step).
 // A step's pieces are requested before the next step's rows: loads come back in order, and a wait for the
-// pieces must not be one for those rows (8192 tokens, 4096 -> 14336, rank 64: 200 us a call against 220).
+// pieces must not be one for those rows (8192 tokens, 4096 -> 14336, rank 64, two pieces: 200 us a call against 220).
 // STREAM: dy is read past the caches (kStreamed).
 template <class E, int RT, bool STREAM>
 __global__ void __launch_bounds__(256, RT == 2 ? 1 : 2) gradient_rows_kernel(WeightArgs a)

@@ -24,7 +24,7 @@
 //
 // Bound: memory.  8192 tokens of 32 + 8 heads of 128 in bf16, out of packed rows, with the Hadamard rotation: 168 MB
 // in 32.5 us (5.2 TB/s; a copy of 512 MB runs at 5.4), 2 us of it the rotation; the backward pass 252 MB in 54 us
-// (4.7 TB/s), 4 us of it the sums of the weight gradients.
+// (4.7 TB/s), 4 us of it the sums of the weight gradients.  fp32: 4096 tokens in 33 and 51 us (5.1 and 4.9 TB/s).
 #include <type_traits>
 
 #include "common.hpp"
@@ -99,7 +99,8 @@ __device__ __forceinline__ void unpack_units(const Raw<E> (&r)[2], float (&v)[2]
 
 // Streaming stores: what a pass over a large batch writes is not read again before it would be evicted, and the
 // heads of 8192 tokens took 34.5 us with them against 41.6.  Not for fp32, where one instruction writes every
-// other 16 bytes of a line: 4096 tokens took 62 us with them against 43.
+// other 16 bytes of a line: 8192 tokens take 74 us with them against 66, the backward pass of 4096 tokens 58
+// against 51 (4096 tokens forward 32 against 33).
 template <class E>
 __device__ __forceinline__ void store_unit(E* p, const float (&v)[8])
 {
